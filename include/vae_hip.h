@@ -570,6 +570,64 @@ int vae_adamw_clip_step_elbo(float* params, const float* grads, float* exp_avg, 
                              const float* recon_partial, int n_recon, const float* kl_partial, int n_kl,
                              float kl_weight, float inv_batch, float* out3, void* stream);
 
+/* ---- The same over MANY separate tensors: torch.nn.utils.clip_grad_norm_ and torch.optim.AdamW, vae/training/train.py:310,336,338,
+ *      for models whose parameters are allocations of their own.  fp32 or bf16 parameters and gradients, moments in 32 or in 8 bits.
+ *
+ * State layout: each tensor's state starts on a block of 256 elements of its group's state buffers (`block`, counted in blocks) and
+ * fills n elements of it; the rest of its last block is padding that is zero and stays zero.  No two tensors share a block.
+ * 8-bit moments: one byte per element and one base per block and moment, bases[2 * block] for exp_avg, bases[2 * block + 1] for
+ * exp_avg_sq.  Code c > 0 stands for the fp32 value whose bits are (base + c) << 20, code 0 for zero; exp_avg: c in the low 7
+ * bits, sign in bit 7, 0x80 = not finite; exp_avg_sq: 255 = not finite.
+ * bf16 parameters: remainder[] and the parameter make a 32-bit master, |master| bits = (|param| bits << 16) + remainder. */
+#define VAE_MT_MAX_TENSORS 65536
+#define VAE_MT_MAX_GROUPS 64
+#define VAE_MT_PARAM_BF16 1u
+#define VAE_MT_GRAD_BF16 2u
+typedef struct {
+    void* param;             /* fp32 (or bf16) elements in the order of the state; not read by the norm and the clip */
+    const void* grad;        /* fp32 (or bf16) elements in the same order; vae_multi_clip writes it */
+    long n;                  /* elements; 0: only the step count advances */
+    unsigned block;          /* first block of its state */
+    unsigned slot;           /* place of its step count and scalars; no two tensors of a call share one */
+    unsigned flags;          /* VAE_MT_* */
+    unsigned reserved;
+} vae_mt_tensor;
+typedef struct {
+    unsigned struct_size;    /* = sizeof(vae_mt_group) */
+    int state_bits;          /* 32 or 8 */
+    const vae_mt_tensor* tensors; /* host memory, read before the call returns */
+    int count;
+    int nslots;
+    void* exp_avg;           /* 32 bits: float[nblocks * 256]; 8 bits: uint8[nblocks * 256] */
+    void* exp_avg_sq;
+    short* bases;            /* 8 bits: short[nblocks * 2] */
+    short* remainder;        /* short[nblocks * 256] where a parameter is bf16 */
+    long nblocks;
+    long* steps;             /* device long[nslots]: steps taken; advanced by the call */
+    float* scalars;          /* device scratch, 8 floats per slot */
+    const float* lr_dev;     /* optional device float that is read instead of lr */
+    double lr, beta1, beta2, eps, weight_decay;
+} vae_mt_group;
+/* doubles of the `partial` scratch of a call over `count` tensors */
+int vae_multi_partials(int count);
+/* norm_out = |grad_mul| * L2 norm of all gradients */
+int vae_multi_grad_norm(const vae_mt_tensor* tensors, int count, double* partial, float grad_mul, float* norm_out, void* stream);
+/* grad *= grad_mul * min(1, max_norm / (norm + 1e-6)), in place; norm_out receives the norm before the clip.  A norm that is not
+ * finite behaves as in torch: NaN makes every gradient NaN. */
+int vae_multi_clip(const vae_mt_tensor* tensors, int count, double* partial, float grad_mul, float max_norm, float* norm_out, void* stream);
+/* One AdamW step of every tensor of every group, gradients scaled as by vae_multi_clip first (in registers: they are not
+ * written).  The norm runs over all groups.  max_norm < 0: no clipping, and with norm_out = NULL no norm is taken. */
+int vae_multi_adamw_step(const vae_mt_group* groups, int ngroups, double* partial, float grad_mul, float max_norm, float* norm_out,
+                         void* stream);
+/* out[block * 256 + k] = 32-bit value of parameter element k (master of a bf16 parameter); padding of listed tensors = 0 */
+int vae_multi_master(const vae_mt_tensor* tensors, int count, const short* remainder, float* out, long nblocks, void* stream);
+/* 8-bit moments -> fp32, or (bf16_out) bf16, which holds their values exactly */
+int vae_moments8_unpack(const void* exp_avg_q, const void* exp_avg_sq_q, const short* bases, void* exp_avg, void* exp_avg_sq,
+                        long nblocks, int bf16_out, void* stream);
+/* fp32 moments -> 8 bits, rounded to nearest */
+int vae_moments8_pack(const float* exp_avg, const float* exp_avg_sq, void* exp_avg_q, void* exp_avg_sq_q, short* bases,
+                      long nblocks, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

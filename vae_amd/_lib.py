@@ -114,6 +114,13 @@ SIGNATURES = {
                                    c_double, c_double, c_int, P, P]),
     "vae_adamw_clip_step_elbo": (None, [P, P, P, P, c_long, P, c_float, c_float, c_double, c_double, c_double,
                                         c_double, c_double, c_int, P, P, c_int, P, c_int, c_float, c_float, P, P]),
+    "vae_multi_partials": (c_int, [c_int]),
+    "vae_multi_grad_norm": (None, [P, c_int, P, c_float, P, P]),
+    "vae_multi_clip": (None, [P, c_int, P, c_float, c_float, P, P]),
+    "vae_multi_adamw_step": (None, [P, c_int, P, c_float, c_float, P, P]),
+    "vae_multi_master": (None, [P, c_int, P, P, c_long, P]),
+    "vae_moments8_unpack": (None, [P, P, P, P, P, c_long, c_int, P]),
+    "vae_moments8_pack": (None, [P, P, P, P, P, c_long, P]),
     "vae_permute_f32": (None, [P, P, P, P, c_long, P]),
     "vae_cast_bf16": (None, [P, P, c_long, P]),
     "vae_model_param_count": (c_long, [P]),
@@ -148,6 +155,25 @@ class WgradJob(ctypes.Structure):
                 ("Cin", c_int), ("Cout", c_int), ("nsplit", c_int)]
 
 
+class MtTensor(ctypes.Structure):
+    """mirror of struct vae_mt_tensor (include/vae_hip.h)."""
+    _fields_ = [("param", c_void_p), ("grad", c_void_p), ("n", c_long), ("block", c_uint), ("slot", c_uint), ("flags", c_uint),
+                ("reserved", c_uint)]
+
+
+class MtGroup(ctypes.Structure):
+    """mirror of struct vae_mt_group (include/vae_hip.h)."""
+    _fields_ = [("struct_size", c_uint), ("state_bits", c_int), ("tensors", c_void_p), ("count", c_int), ("nslots", c_int),
+                ("exp_avg", c_void_p), ("exp_avg_sq", c_void_p), ("bases", c_void_p), ("remainder", c_void_p),
+                ("nblocks", c_long), ("steps", c_void_p), ("scalars", c_void_p), ("lr_dev", c_void_p),
+                ("lr", c_double), ("beta1", c_double), ("beta2", c_double), ("eps", c_double), ("weight_decay", c_double)]
+
+    def __init__(self, *args, **kw):
+        super().__init__(*args, **kw)
+        self.struct_size = ctypes.sizeof(MtGroup)       # the library compares it with its own sizeof(vae_mt_group)
+
+
+MT_PARAM_BF16, MT_GRAD_BF16, MT_BLOCK, MT_MAX_GROUPS, MT_MAX_TENSORS = 1, 2, 256, 64, 65536      # VAE_MT_* of include/vae_hip.h
 ABI_VERSION = 3                          # VAE_HIP_VERSION of the include/vae_hip.h these signatures were written for
 PRECISIONS = {"bf16": 0, "fp32": 1}      # VAE_PRECISION_* of include/vae_hip.h
 

@@ -16,6 +16,7 @@ import torch.nn.functional as F
 import yaml
 
 from . import _lib
+from .optim import MultiAdamW
 
 # "bce_logits" is the draft script's vae_loss_bce (vae/practice/vae_conv.py:146-151): logits clamped to [-10, 10]
 # first, no gradient outside.  The torch callable itself is unclamped ("bce_logits_raw").
@@ -161,9 +162,18 @@ def train_step(model, optimizer, inputs, config, eps=None, keep_masks=None, max_
     kind = recon_kind_from_config(config)
     loss = _ElboLoss.apply(recons, inputs, mu, logvar, kind, float(config.kl_weight))
     loss.backward()
-    torch.nn.utils.clip_grad_norm_(model.parameters(), max_norm=max_norm)
-    optimizer.step()
+    _clip_and_step(model, optimizer, max_norm)
     return loss.detach()
+
+
+def _clip_and_step(model, optimizer, max_norm):
+    """clip_grad_norm_(max_norm); optimizer.step() (train.py:336-338).  MultiAdamW clips while it steps, provided that it steps all
+    of the model's parameters: the norm runs over those it holds."""
+    if isinstance(optimizer, MultiAdamW) and optimizer.holds(model.parameters()):
+        optimizer.step(max_norm=max_norm)
+    else:
+        torch.nn.utils.clip_grad_norm_(model.parameters(), max_norm=max_norm)
+        optimizer.step()
 
 
 def val_step(model, inputs, config, eps=None):
@@ -226,8 +236,7 @@ class FusedStep:
         else:
             for p, g in zip(m._ordered_params(), self._grad_views):
                 p.grad = g
-            torch.nn.utils.clip_grad_norm_(m.parameters(), max_norm=self.max_norm)
-            self.optimizer.step()
+            _clip_and_step(m, self.optimizer, self.max_norm)
             m.repack_weights()        # the torch optimizer wrote the fp32 parameters: refresh the bf16 operand copies
         # only now: the optimizer's first launch reads the KL partial sums out of this workspace (`elbo`), so the buffer
         # must not go back to the pool (where the next forward of any caller would take it) before that launch is queued

@@ -581,6 +581,7 @@ int vae_adamw_clip_step_elbo(float* params, const float* grads, float* exp_avg, 
  * bf16 parameters: remainder[] and the parameter make a 32-bit master, |master| bits = (|param| bits << 16) + remainder. */
 #define VAE_MT_MAX_TENSORS 65536
 #define VAE_MT_MAX_GROUPS 64
+#define VAE_MT_MIN_EPS8 1e-12    /* smallest eps of a group with 8-bit moments */
 #define VAE_MT_PARAM_BF16 1u
 #define VAE_MT_GRAD_BF16 2u
 typedef struct {

@@ -19,8 +19,10 @@ def adamw(p, g, m, v, t, lr=1e-4, b1=0.9, b2=0.999, eps=1e-8, wd=0.01, coef=1.0)
     """step t in 64 bits: (p, m, v) and a bound on each one's error in fp32 arithmetic.  Roundings counted per operation, half a step each:
     m: coef, coef g, the constants' own rounding (2), two products, the sum: at most 6 halves of |b1 m| + |(1 - b1) g|.
     v: the same with g squared (coef and coef g count twice, one product more): 10 halves.
-    the step: lr and the bias corrections rounded (2), product, root, its factor, sum with eps (rounded itself), division: 8 halves,
-    plus m's error over the divisor and half of v's relative error; then decay (2), product and difference of p."""
+    the step: lr and the bias corrections rounded (2), product, root, its factor, sum with eps (rounded itself), division: 8 halves.
+    With 8-bit moments root and reciprocal are the hardware's, off by a whole last place each (2 halves instead of 1, the reciprocal's
+    product 1 more; root's factor and sum are one operation, 1 less): step size, product, 2 root + factor rounded, sum, 2 + 1: 9 halves.
+    Plus m's error over the divisor and half of v's relative error (5 halves): 14; then decay (2), product and difference of p."""
     p, g, m, v = (np.asarray(x, np.float64) for x in (p, g, m, v))
     g = g * coef
     m1, v1 = b1 * m + (1 - b1) * g, b2 * v + (1 - b2) * g * g
@@ -29,7 +31,7 @@ def adamw(p, g, m, v, t, lr=1e-4, b1=0.9, b2=0.999, eps=1e-8, wd=0.01, coef=1.0)
     den = np.sqrt(v1) / np.sqrt(1 - b2 ** t) + eps
     step = lr / (1 - b1 ** t) * m1 / den
     p1 = p * (1 - lr * wd) - step
-    dp = EPS24 * (3 * np.abs(p) + np.abs(p1) + 13 * np.abs(step)) + lr / (1 - b1 ** t) * dm / den
+    dp = EPS24 * (3 * np.abs(p) + np.abs(p1) + 14 * np.abs(step)) + lr / (1 - b1 ** t) * dm / den
     return (p1, m1, v1), (dp, dm, dv)
 
 

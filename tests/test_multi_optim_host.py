@@ -64,7 +64,7 @@ def test_norm_and_clip_refuse_scratch_and_counts():
 
 @pytest.mark.parametrize("jobs, kw, match", [
     ([job()], dict(state_bits=16), "state_bits"), ([job()], dict(beta1=1.0), "betas"), ([job()], dict(beta2=-0.1), "betas"),
-    ([job()], dict(eps=-1.0), "eps"), ([job()], dict(lr=-1.0), "lr"), ([job()], dict(weight_decay=float("nan")), "weight_decay"),
+    ([job()], dict(eps=-1.0), "eps"), ([job()], dict(state_bits=8, eps=1e-13, bases=4096), "8-bit moments need"), ([job()], dict(lr=-1.0), "lr"), ([job()], dict(weight_decay=float("nan")), "weight_decay"),
     ([job()], dict(exp_avg=None), "null state"), ([job()], dict(state_bits=8), "null state"), ([job()], dict(exp_avg=4100), "16-byte"),
     ([job()], dict(steps=None), "step counts"), ([job(n=1025)], {}, "reaches behind"), ([job(block=4)], {}, "reaches behind"),
     ([job(slot=1)], {}, "slot"), ([job(param=None)], {}, "parameter is null"), ([job(param=4098)], {}, "not aligned"),
@@ -135,7 +135,7 @@ def test_python_layer_refuses_on_the_cpu():
 @pytest.mark.parametrize("kw, match", [
     (dict(lr=-1.0), "lr"), (dict(betas=(1.0, 0.9)), "betas"), (dict(betas=(0.9, -0.1)), "betas"), (dict(eps=-1e-8), "eps"),
     (dict(weight_decay=-1.0), "weight_decay"), (dict(state_bits=16), "state_bits"), (dict(lr=torch.tensor(1e-3)), "on the GPU"),
-    (dict(lr=float("nan")), "lr")])
+    (dict(lr=float("nan")), "lr"), (dict(eps=0.0, state_bits=8), "8-bit moments need")])
 def test_python_layer_refuses_hyperparameters(kw, match):
     with pytest.raises(ValueError, match=match):
         optim.MultiAdamW([cpu_param(4)], **kw)

@@ -37,8 +37,19 @@ namespace vae {
 
 #define MT_TENSORS 192           // tensors one launch takes: 32 + 4 bytes of kernel arguments each
 #define MT_CHUNK 4096            // elements a workgroup takes at a time
+#define AD_DEEP 4                // blocks a wave of the step has in flight
 #define MT_BLOCK 256             // elements of one tensor that share a base; a wave's 64 lanes x 4
-#define MT_PARTIALS 256          // workgroups (= partial sums) of the norm; every launch of a longer list has at least one
+#define MT_PARTIALS 256          // workgroups (= partial sums) of the norm, one per CU; every launch of a longer list has at least one
+#define SQ_THREADS 1024
+#define SQ_DEEP 4                // 16-byte loads a thread of the norm has in flight
+#define SQ_CHUNK (SQ_THREADS * SQ_DEEP * 4)
+
+// The moments and remainders of a step whose tensors and state are larger than this are loaded and stored past the caches: the last
+// level holds 256 MB, what is larger is gone before the next step reads it.  69.8 M parameters (1.1 GB): 347 us against 377, with
+// 8-bit moments (0.7 GB) 188 against 208; 4.1 M parameters (65 MB), which do stay: 26 us against 22.  Parameters and gradients stay
+// cached in any case: the norm has just read the gradients, the next forward pass reads the parameters (bf16, 20 M of
+// them: 96 us against 107 past the caches too; fp32 no difference).
+#define MT_STREAM_BYTES 256e6
 
 struct MtJob {
     void* p;
@@ -73,6 +84,15 @@ struct MtScal {
     uint32_t phase_m, phase_v;
 };
 
+// one chunk's addresses
+struct MtChunk {
+    void* p;
+    const void* g;
+    void *m, *v;
+    short* rem;
+    short2* base;
+};
+
 #define DITHER_I 0x9E3779B9u     // 2^32 / golden ratio
 #define DITHER_M 0xBB67AE85u     // 2^32 * frac(sqrt 3)
 #define DITHER_V 0x6A09E667u     // 2^32 * frac(sqrt 2)
@@ -96,62 +116,98 @@ struct MtFind {
     }
 };
 
-// four consecutive elements from index i of n; elements behind the end read as 0
-template <bool BF>
-__device__ __forceinline__ void load4(const void* p, long i, long n, float x[4]) {
-    if (i + 4 <= n) {
-        if (BF) {
-            const u16x4u q = *(const u16x4u*)((const bf16_t*)p + i);
+// NT: a streaming access, which the caches need not keep
+template <bool NT, class T>
+__device__ __forceinline__ T ld(const T* p) {
+    if (NT) return __builtin_nontemporal_load(p);
+    return *p;
+}
+template <bool NT, class T>
+__device__ __forceinline__ void st(T* p, T x) {
+    if (NT) __builtin_nontemporal_store(x, p);
+    else *p = x;
+}
+
+// four consecutive elements at p + o, of which the tensor has `left` (FULL: four); what it has not reads as 0 and is not written
+template <bool FULL>
+__device__ __forceinline__ void load4(const float* p, uint32_t o, int left, float x[4]) {
+    if (FULL || left >= 4) {
+        const f32x4u q = *(const f32x4u*)(p + o);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = bf2f(q[k]);
-        } else {
-            const f32x4u q = *(const f32x4u*)((const float*)p + i);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = q[k];
-        }
+        for (int k = 0; k < 4; ++k) x[k] = q[k];
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = i + k < n ? (BF ? bf2f(((const bf16_t*)p)[i + k]) : ((const float*)p)[i + k]) : 0.f;
+        for (int k = 0; k < 4; ++k) x[k] = k < left ? p[o + k] : 0.f;
     }
 }
-__device__ __forceinline__ void store4(float* p, long i, long n, const float x[4]) {
-    if (i + 4 <= n) {
+template <bool FULL>
+__device__ __forceinline__ void load4(const bf16_t* p, uint32_t o, int left, u16x4u& x) {
+    if (FULL || left >= 4) {
+        x = *(const u16x4u*)(p + o);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = k < left ? p[o + k] : (bf16_t)0;
+    }
+}
+template <bool BF, bool FULL>
+__device__ __forceinline__ void load4(const void* p, uint32_t o, int left, float x[4]) {
+    if (BF) {
+        u16x4u q;
+        load4<FULL>((const bf16_t*)p, o, left, q);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = bf2f(q[k]);
+    } else {
+        load4<FULL>((const float*)p, o, left, x);
+    }
+}
+template <bool FULL>
+__device__ __forceinline__ void store4(float* p, uint32_t o, int left, const float x[4]) {
+    if (FULL || left >= 4) {
         f32x4u q;
 #pragma unroll
         for (int k = 0; k < 4; ++k) q[k] = x[k];
-        *(f32x4u*)(p + i) = q;
+        *(f32x4u*)(p + o) = q;
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-            if (i + k < n) p[i + k] = x[k];
+            if (k < left) p[o + k] = x[k];
     }
 }
-__device__ __forceinline__ void store4(bf16_t* p, long i, long n, const bf16_t x[4]) {
-    if (i + 4 <= n) {
+template <bool FULL>
+__device__ __forceinline__ void store4(bf16_t* p, uint32_t o, int left, const bf16_t x[4]) {
+    if (FULL || left >= 4) {
         u16x4u q;
 #pragma unroll
         for (int k = 0; k < 4; ++k) q[k] = x[k];
-        *(u16x4u*)(p + i) = q;
+        *(u16x4u*)(p + o) = q;
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-            if (i + k < n) p[i + k] = x[k];
+            if (k < left) p[o + k] = x[k];
     }
 }
 
 // ---------------------------------------------------------------- global norm
 // Squares and sums in 64 bits: a square of an fp32 gradient can pass fp32's range, and the sum runs over the whole model.
+// Bound by HBM, 4 bytes a gradient.  One workgroup of 16 waves per CU, so that every wave of the kernels that read the norm
+// folds 256 partial sums (four loads a lane) and needs no launch of its own for that.  279 MB in 88 tensors: 48 us, 5.8 TB/s;
+// with 256 threads a workgroup 160 us, with 512 or 1024 workgroups of 256 to 1024 threads and up to 8 loads in flight 47 to 53.
 template <bool BF>
-__device__ __forceinline__ double sumsq_chunk(const void* g, long c0, long n) {
-    double a = 0.0;
-    float x[4][4];
+__device__ __forceinline__ void sumsq_chunk(const void* g, long c0, long n, double a[4]) {
+    const void* p = (const char*)g + c0 * (BF ? 2 : 4);
+    const int left = (int)(n - c0 < SQ_CHUNK ? n - c0 : SQ_CHUNK);
+    float x[SQ_DEEP][4];
+    if (left == SQ_CHUNK) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) load4<BF>(g, c0 + (u * 256 + (int)threadIdx.x) * 4L, n, x[u]);
+        for (int u = 0; u < SQ_DEEP; ++u) load4<BF, true>(p, (u * SQ_THREADS + threadIdx.x) * 4u, 0, x[u]);
+    } else {
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < SQ_DEEP; ++u) load4<BF, false>(p, (u * SQ_THREADS + threadIdx.x) * 4u, left - (int)((u * SQ_THREADS + threadIdx.x) * 4u), x[u]);
+    }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) a = __builtin_fma((double)x[u][k], (double)x[u][k], a);
-    return a;
+    for (int u = 0; u < SQ_DEEP; ++u)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a[k] = __builtin_fma((double)x[u][k], (double)x[u][k], a[k]);
 }
 
 // beta^t, t >= 1, by squaring: 2 log2(t) multiplications, off by less than t * 2^-53 of its value
@@ -183,24 +239,29 @@ __device__ __forceinline__ void prep_tensors(const MtTable& tab, const MtPrep& h
 
 // workgroups 0..nsum-1: partial sums; with PREP one more, which prepares the step of the same tensors
 template <bool PREP>
-__global__ __launch_bounds__(256) void multi_sumsq_kernel(const MtTable tab, double* __restrict__ partial, int nsum, const MtPrep prep) {
+__global__ __launch_bounds__(SQ_THREADS) void multi_sumsq_kernel(const MtTable tab, double* __restrict__ partial, int nsum, const MtPrep prep) {
     if (PREP && (int)blockIdx.x >= nsum) {
         prep_tensors(tab, prep);
         return;
     }
-    __shared__ double red[4];
+    __shared__ double red[SQ_THREADS / 64];
     const MtFind find(tab);
-    double a = 0.0;
+    double a4[4] = {0.0, 0.0, 0.0, 0.0};
     for (uint32_t c = blockIdx.x; c < tab.nchunk; c += nsum) {
         const int j = find(c);
         const MtJob& jb = tab.job[j];
-        const long c0 = (long)(c - tab.first[j]) * MT_CHUNK;
-        a += (jb.slot_flags & VAE_MT_GRAD_BF16) ? sumsq_chunk<true>(jb.g, c0, jb.n) : sumsq_chunk<false>(jb.g, c0, jb.n);
+        const long c0 = (long)(c - tab.first[j]) * SQ_CHUNK;
+        if (jb.slot_flags & VAE_MT_GRAD_BF16) sumsq_chunk<true>(jb.g, c0, jb.n, a4);
+        else sumsq_chunk<false>(jb.g, c0, jb.n, a4);
     }
-    a = wave_sum_d(a);
+    const double a = wave_sum_d((a4[0] + a4[1]) + (a4[2] + a4[3]));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
     __syncthreads();
-    if (threadIdx.x == 0) partial[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+    if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int w = 0; w < SQ_THREADS / 64; ++w) t += red[w];
+        partial[blockIdx.x] = t;
+    }
 }
 
 struct MtClip {
@@ -224,25 +285,31 @@ __device__ __forceinline__ float clip_coef(const MtClip& c) {
     return (float)(q >= 1.0 ? 1.0 : q) * c.grad_mul;
 }
 
-template <bool BF>
-__device__ __forceinline__ void scale_chunk(void* g, long c0, long n, float coef) {
+template <bool BF, bool FULL>
+__device__ __forceinline__ void scale_run(void* g, int left, float coef) {
     float x[4][4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) load4<BF>(g, c0 + (u * 256 + (int)threadIdx.x) * 4L, n, x[u]);
+    for (int u = 0; u < 4; ++u) load4<BF, FULL>(g, (u * 256 + threadIdx.x) * 4u, left - (int)((u * 256 + threadIdx.x) * 4u), x[u]);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-        const long i = c0 + (u * 256 + (int)threadIdx.x) * 4L;
+        const uint32_t o = (u * 256 + threadIdx.x) * 4u;
         if (BF) {
             bf16_t y[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) y[k] = f2bf(x[u][k] * coef);
-            store4((bf16_t*)g, i, n, y);
+            store4<FULL>((bf16_t*)g, o, left - (int)o, y);
         } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k) x[u][k] *= coef;
-            store4((float*)g, i, n, x[u]);
+            store4<FULL>((float*)g, o, left - (int)o, x[u]);
         }
     }
+}
+template <bool BF>
+__device__ __forceinline__ void scale_chunk(void* g, long c0, long n, float coef) {
+    void* p = (char*)g + c0 * (BF ? 2 : 4);
+    if (n - c0 >= MT_CHUNK) scale_run<BF, true>(p, MT_CHUNK, coef);
+    else scale_run<BF, false>(p, (int)(n - c0), coef);
 }
 
 __global__ __launch_bounds__(256) void multi_scale_kernel(const MtTable tab, const MtClip clip) {
@@ -260,10 +327,17 @@ __global__ __launch_bounds__(256) void multi_scale_kernel(const MtTable tab, con
 __global__ __launch_bounds__(64) void multi_norm_kernel(const MtClip clip) { clip_coef(clip); }
 
 // ---------------------------------------------------------------- 8-bit moments
+// maximum over the wave, in a scalar register: within rows of 16 lanes, then across them, towards lane 63
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
-    return v;
+#define MT_DPP_MAX(ctrl, rows) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, false))
+    MT_DPP_MAX(0x111, 0xF);      // row_shr:1, 2, 4, 8
+    MT_DPP_MAX(0x112, 0xF);
+    MT_DPP_MAX(0x114, 0xF);
+    MT_DPP_MAX(0x118, 0xF);
+    MT_DPP_MAX(0x142, 0xA);      // row_bcast:15, 31
+    MT_DPP_MAX(0x143, 0xC);
+#undef MT_DPP_MAX
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 __device__ __forceinline__ bool finite_bits(uint32_t x) { return x < 0x7F800000u; }     // of a magnitude
 __device__ __forceinline__ int level_up(uint32_t x) { return min((int)((x + 0xFFFFFu) >> 20), 0x7F7); }
@@ -278,136 +352,210 @@ __device__ __forceinline__ float unpack_v(uint32_t q, int base) {
     const uint32_t x = q ? (uint32_t)(base + (int)q) << 20 : 0u;
     return __uint_as_float(q == 255u ? 0x7FC00000u : x);
 }
-// low: level base + 1, the smallest that has a code.  Below it the value becomes 0 or that level, the latter with
-// probability |m| / low over the dither (d * low is exact: 20 bits times 4)
-__device__ __forceinline__ uint32_t pack_m(float m, int base, float low, uint32_t d) {
-    const uint32_t x = __float_as_uint(m) & 0x7FFFFFFFu;
-    const float a = __uint_as_float(x);
-    const uint32_t big = (uint32_t)min((int)((x + d) >> 20) - base, 127);
-    const uint32_t c = a >= low ? big : (a > (float)d * (low * 0x1p-20f) ? 1u : 0u);
-    const uint32_t q = c ? c | ((__float_as_uint(m) >> 24) & 128u) : 0u;
-    return finite_bits(x) ? q : 128u;
+// Does one of the four codes of a word mean "not finite"?  (a byte of x is zero: (x - 01..01) & ~x & 80..80 is not)
+__device__ __forceinline__ bool odd_codes(uint32_t qm, uint32_t qv) {
+    const uint32_t a = qm ^ 0x80808080u;
+    return (((a - 0x01010101u) & ~a) | ((~qv - 0x01010101u) & qv)) & 0x80808080u;
 }
-__device__ __forceinline__ uint32_t pack_v(float v, int base, uint32_t d) {
-    const uint32_t x = __float_as_uint(v) & 0x7FFFFFFFu;
-    const int c = min(max((int)((x + d) >> 20) - base, 1), 254);
-    return finite_bits(x) ? (x ? (uint32_t)c : 0u) : 255u;
-}
-
-// bases of a wave's block from each lane's four values; every lane gets them
-__device__ __forceinline__ void block_bases(const float m[4], const float v[4], int& bm, int& bv) {
-    uint32_t xm = 0, xv = 0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const uint32_t a = __float_as_uint(m[k]) & 0x7FFFFFFFu, b = __float_as_uint(v[k]) & 0x7FFFFFFFu;
-        xm = max(xm, finite_bits(a) ? a : 0u);
-        xv = max(xv, finite_bits(b) ? b : 0u);
-    }
-    bm = max(level_up(wave_max_u32(xm)) - 127, 0);
-    bv = max(level_up(wave_max_u32(xv)) - 254, 0);
-}
-__device__ __forceinline__ uint32_t pack_base(int bm, int bv) { return (uint32_t)bm | (uint32_t)bv << 16; }
 
 // ---------------------------------------------------------------- AdamW
-// (parameter, remainder) <-> master; a magnitude below zero can only come of a parameter that was written since, and is 0
+// (parameter, remainder) -> master.  A magnitude below zero can only come of a parameter that was written since, and is 0.
 __device__ __forceinline__ float join_master(bf16_t p, short r) {
-    const uint32_t hi = (uint32_t)(p & 0x7FFF) << 16;
-    const uint32_t x = hi >= 0x7F800000u && (r > 0 || hi > 0x7F800000u) ? hi : (uint32_t)max((int)hi + (int)r, 0);
-    return __uint_as_float(x | (uint32_t)(p & 0x8000) << 16);
+    const uint32_t t = (uint32_t)p << 16;
+    const uint32_t x = (uint32_t)max((int)(t & 0x7FFF0000u) + (int)r, 0);
+    return __uint_as_float(x | (t & 0x80000000u));
 }
+// master -> (parameter, remainder): adding half a last place rounds the magnitude, and what the upper half is then too
+// large or too small by is the lower half, read as a signed number
 __device__ __forceinline__ void split_master(float w, bf16_t& p, short& r) {
-    const uint32_t x = __float_as_uint(w) & 0x7FFFFFFFu;
-    const uint32_t hi = x > 0x7F800000u ? 0x7FC0u : (x + 0x8000u) >> 16;
-    r = x > 0x7F800000u ? (short)0 : (short)(int)(x - (hi << 16));
-    p = (bf16_t)(hi | ((__float_as_uint(w) >> 16) & 0x8000u));
+    const uint32_t x = w != w ? 0x7FC00000u : __float_as_uint(w);
+    p = (bf16_t)((x + 0x8000u) >> 16);
+    r = (short)(x & 0xFFFFu);
 }
 
-// One block of 256 elements (a wave: 4 per lane) of one tensor.
-template <bool PB, bool GB, bool S8>
-__device__ __forceinline__ void adamw_block(const MtJob& jb, const MtHyper& h, const MtScal& s, float coef, long i, long blk, int lane) {
-    const size_t k0 = (size_t)blk * MT_BLOCK + lane * 4;
+// One block of 256 elements of one tensor, a wave's work: 4 elements a lane.  All of a wave's blocks of a chunk are loaded before the
+// first is stored: the stores could alias the later loads as far as the compiler knows, and would wait for one another.
+// Bound by HBM: 28 bytes a parameter in fp32 with 32-bit moments, 16 with 8-bit ones (26 and 14 in bf16 with remainder).
+// 69.8 M fp32 parameters in 88 tensors: 341 us, 5.7 TB/s; 8-bit moments 192 us, 5.8 TB/s (a pass over one array in place
+// reaches 5.9).  20 M bf16 parameters in 217 tensors off their alignment: 86 us, 6.0 TB/s.
+//
+// In 8 bits the vector instructions count: 16 bytes a parameter at 5.9 TB/s leave about 100 of them.  The first form took
+// 110 a parameter and 240 us, this one 66 (bf16: 81).  So
+// - root and reciprocal are the hardware's, 1 ulp each, of a step that is itself a small part of the parameter.  The hardware takes
+//   the root of a subnormal for 0, which nobody sees next to an eps of at least 1e-12 (VAE_MT_MIN_EPS8): smaller ones are refused;
+// - values that are not finite, their codes, and fp32's last level are looked after in branches that a wave seldom takes;
+// - a block's maxima go through the lanes by DPP and end in scalar registers, where the bases are worked out;
+// - a full chunk has uniform addresses and no bounds; only a tensor's last chunk looks at its end.
+template <bool PB, bool GB, bool S8, bool NT>
+struct AdamBlock {
     float p[4], g[4], m[4], v[4];
-    load4<GB>(jb.g, i, jb.n, g);
-    if (PB) {
-        u16x4u q = {0, 0, 0, 0};
-        if (i + 4 <= jb.n) q = *(const u16x4u*)((const bf16_t*)jb.p + i);
-        else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (i + k < jb.n) q[k] = ((const bf16_t*)jb.p)[i + k];
+    uint32_t qm, qv, base;
+    short4v r;
+    u16x4u pb;
+
+    // o: this lane's first element, counted from the chunk's start; left: elements of the tensor from there on (FULL: at least the
+    // whole chunk)
+    template <bool FULL>
+    __device__ __forceinline__ void load(const MtChunk& c, uint32_t o, int left) {
+        load4<GB, FULL>(c.g, o, left, g);
+        if (PB) {
+            load4<FULL>((const bf16_t*)c.p, o, left, pb);
+            r = ld<NT>((const short4v*)(c.rem + o));
+        } else {
+            load4<false, FULL>(c.p, o, left, p);
         }
-        const short4v r = *(const short4v*)(h.rem + k0);
+        if (S8) {
+            qm = ld<NT>((const uint32_t*)((const uint8_t*)c.m + o));
+            qv = ld<NT>((const uint32_t*)((const uint8_t*)c.v + o));
+            base = *(const uint32_t*)(c.base + o / MT_BLOCK);
+        } else {
+            const f32x4 a = ld<NT>((const f32x4*)((const float*)c.m + o)), b = ld<NT>((const f32x4*)((const float*)c.v + o));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) p[k] = join_master(q[k], r[k]);
-    } else {
-        load4<false>(jb.p, i, jb.n, p);
+            for (int k = 0; k < 4; ++k) { m[k] = a[k]; v[k] = b[k]; }
+        }
     }
-    if (S8) {
-        const uint32_t qm = *(const uint32_t*)((const uint8_t*)h.m + k0), qv = *(const uint32_t*)((const uint8_t*)h.v + k0);
-        const short2 b = h.base[blk];
+
+    __device__ __forceinline__ void unpack() {
+        const uint32_t b = (uint32_t)__builtin_amdgcn_readfirstlane((int)base), bm = b & 0xFFFFu, bv = b >> 16;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            m[k] = unpack_m((qm >> 8 * k) & 255u, b.x);
-            v[k] = unpack_v((qv >> 8 * k) & 255u, b.y);
+            const uint32_t cm = (qm >> 8 * k) & 127u, cv = (qv >> 8 * k) & 255u;
+            m[k] = __uint_as_float((cm ? (cm + bm) << 20 : 0u) | ((qm << (24 - 8 * k)) & 0x80000000u));
+            v[k] = __uint_as_float(cv ? (cv + bv) << 20 : 0u);
         }
-    } else {
-        const f32x4 a = *(const f32x4*)((const float*)h.m + k0), b = *(const f32x4*)((const float*)h.v + k0);
+        if (__any(odd_codes(qm, qv))) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) { m[k] = a[k]; v[k] = b[k]; }
+            for (int k = 0; k < 4; ++k) {
+                if (((qm >> 8 * k) & 255u) == 128u) m[k] = __uint_as_float(0x7FC00000u);
+                if (((qv >> 8 * k) & 255u) == 255u) v[k] = __uint_as_float(0x7FC00000u);
+            }
+        }
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const float gk = g[k] * coef;
-        m[k] = h.b1 * m[k] + h.omb1 * gk;
-        v[k] = h.b2 * v[k] + h.omb2 * gk * gk;
-        p[k] = p[k] * s.decay - s.step * m[k] / (sqrtf(v[k]) * s.inv_bc2 + h.eps);
-    }
-    if (PB) {
-        bf16_t q[4];
-        short4v r;
+
+    // codes of m and v (which it may change); returns the bases.  i: index of the first element; NEAR: to nearest, without a dither
+    template <bool NEAR>
+    __device__ __forceinline__ uint32_t pack(uint32_t phase_m, uint32_t phase_v, uint32_t i) {
+        uint32_t xm = 0, xv = 0, odd_m = 0, odd_v = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            short rk;
-            split_master(p[k], q[k], rk);
-            r[k] = i + k < jb.n ? rk : (short)0;
+            xm = max(xm, __float_as_uint(m[k]) & 0x7FFFFFFFu);
+            xv = max(xv, __float_as_uint(v[k]) & 0x7FFFFFFFu);
         }
-        store4((bf16_t*)jb.p, i, jb.n, q);
-        *(short4v*)(h.rem + k0) = r;
-    } else {
-        store4((float*)jb.p, i, jb.n, p);
-    }
-    if (S8) {
-        int bm, bv;
-        block_bases(m, v, bm, bv);
-        const float low = __uint_as_float((uint32_t)(bm + 1) << 20);
-        uint32_t qm = 0, qv = 0, u = (uint32_t)i * DITHER_I;
+        if (__any(max(xm, xv) >= 0x7F700000u)) {
+            // not finite: packed as 0 and marked afterwards; fp32's last level: has no level above it to be rounded to
+            xm = xv = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t x = __float_as_uint(m[k]) & 0x7FFFFFFFu, y = __float_as_uint(v[k]) & 0x7FFFFFFFu;
+                if (!finite_bits(x)) { odd_m |= 128u << 8 * k; m[k] = 0.f; }
+                else if (x > 0x7F700000u) m[k] = copysignf(__uint_as_float(0x7F700000u), m[k]);
+                if (!finite_bits(y)) { odd_v |= 255u << 8 * k; v[k] = 0.f; }
+                else v[k] = __uint_as_float(min(y, 0x7F700000u));
+                xm = max(xm, __float_as_uint(m[k]) & 0x7FFFFFFFu);
+                xv = max(xv, __float_as_uint(v[k]));
+            }
+        }
+        const uint32_t bm = (uint32_t)max(level_up(wave_max_u32(xm)) - 127, 0), bv = (uint32_t)max(level_up(wave_max_u32(xv)) - 254, 0);
+        const float low = __uint_as_float((bm + 1) << 20), unit = low * 0x1p-20f;
+        uint32_t u = i * DITHER_I;
+        qm = odd_m;
+        qv = odd_v;
 #pragma unroll
         for (int k = 0; k < 4; ++k, u += DITHER_I) {
-            qm |= pack_m(m[k], bm, low, (u + s.phase_m) >> 12) << 8 * k;
-            qv |= pack_v(v[k], bv, (u + s.phase_v) >> 12) << 8 * k;
+            const uint32_t x = __float_as_uint(m[k]) & 0x7FFFFFFFu, y = __float_as_uint(v[k]);
+            const uint32_t dm = NEAR ? 1u << 19 : (u + phase_m) >> 12, dv = NEAR ? 1u << 19 : (u + phase_v) >> 12;
+            const float a = __uint_as_float(x);
+            // below the smallest level that has a code: 0 or that level, the latter with probability |m| / low over the
+            // dither (d * unit is exact: 20 bits times 4)
+            uint32_t c = a > (float)dm * unit ? 1u : 0u;
+            c = a >= low ? ((x + dm) >> 20) - bm : c;
+            qm |= (c ? c | ((__float_as_uint(m[k]) >> 24) & 128u) : 0u) << 8 * k;
+            const uint32_t e = (uint32_t)max((int)((y + dv) >> 20) - (int)bv, 1);
+            qv |= (y ? e : 0u) << 8 * k;
         }
-        *(uint32_t*)((uint8_t*)h.m + k0) = qm;
-        *(uint32_t*)((uint8_t*)h.v + k0) = qv;
-        if (lane == 0) *(uint32_t*)(h.base + blk) = pack_base(bm, bv);
-    } else {
-        const f32x4 a = {m[0], m[1], m[2], m[3]}, b = {v[0], v[1], v[2], v[3]};
-        *(f32x4*)((float*)h.m + k0) = a;
-        *(f32x4*)((float*)h.v + k0) = b;
+        return bm | bv << 16;
     }
-}
 
-template <bool PB, bool GB, bool S8>
-__device__ __forceinline__ void adamw_chunk(const MtJob& jb, const MtHyper& h, const MtScal& s, float coef, long c0) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // i: index of the first element in its tensor
+    template <bool FULL>
+    __device__ __forceinline__ void step(const MtChunk& c, const MtHyper& h, const MtScal& s, float coef, uint32_t o, int left, uint32_t i) {
+        if (PB) {
 #pragma unroll
-    for (int u = 0; u < MT_CHUNK / MT_BLOCK / 4; ++u) {
-        const long b0 = c0 + (u * 4 + wave) * MT_BLOCK;
-        if (b0 >= jb.n) break;
-        adamw_block<PB, GB, S8>(jb, h, s, coef, b0 + lane * 4, jb.block + b0 / MT_BLOCK, lane);
+            for (int k = 0; k < 4; ++k) p[k] = join_master(pb[k], r[k]);
+        }
+        if (S8) unpack();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {      // m and v: one rounding per operation, as the plain formula has them
+            const float gk = g[k] * coef;
+            m[k] = h.b1 * m[k] + h.omb1 * gk;
+            v[k] = h.b2 * v[k] + h.omb2 * gk * gk;
+        }
+        if (S8) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float den = __builtin_fmaf(__builtin_amdgcn_sqrtf(v[k]), s.inv_bc2, h.eps);
+                p[k] = __builtin_fmaf(p[k], s.decay, -(s.step * m[k] * __builtin_amdgcn_rcpf(den)));
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) p[k] = p[k] * s.decay - s.step * m[k] / (sqrtf(v[k]) * s.inv_bc2 + h.eps);
+        }
+        if (PB) {
+            bf16_t q[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                short rk;
+                split_master(p[k], q[k], rk);
+                r[k] = rk;
+            }
+            store4<FULL>((bf16_t*)c.p, o, left, q);
+            st<NT>((short4v*)(c.rem + o), r);
+        } else {
+            store4<FULL>((float*)c.p, o, left, p);
+        }
+        if (S8) {
+            const uint32_t bases = pack<false>(s.phase_m, s.phase_v, i);
+            st<NT>((uint32_t*)((uint8_t*)c.m + o), qm);
+            st<NT>((uint32_t*)((uint8_t*)c.v + o), qv);
+            if ((o & (MT_BLOCK - 1)) == 0) *(uint32_t*)(c.base + o / MT_BLOCK) = bases;
+        } else {
+            st<NT>((f32x4*)((float*)c.m + o), f32x4{m[0], m[1], m[2], m[3]});
+            st<NT>((f32x4*)((float*)c.v + o), f32x4{v[0], v[1], v[2], v[3]});
+        }
+    }
+};
+
+template <bool PB, bool GB, bool S8, bool NT>
+__device__ __forceinline__ void adamw_chunk(const MtJob& jb, const MtHyper& h, const MtScal& s, float coef, long c0) {
+    const size_t k0 = (size_t)jb.block * MT_BLOCK + c0;
+    const MtChunk c = {(char*)jb.p + c0 * (PB ? 2 : 4), (const char*)jb.g + c0 * (GB ? 2 : 4), (char*)h.m + k0 * (S8 ? 1 : 4),
+                       (char*)h.v + k0 * (S8 ? 1 : 4), h.rem + k0, h.base + k0 / MT_BLOCK};
+    const uint32_t lane4 = (threadIdx.x & 63) * 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i0 = (uint32_t)c0;
+    if (jb.n - c0 >= MT_CHUNK) {
+#pragma unroll 1
+        for (uint32_t b = wave * MT_BLOCK; b < MT_CHUNK; b += 4 * AD_DEEP * MT_BLOCK) {
+            AdamBlock<PB, GB, S8, NT> a[AD_DEEP];
+#pragma unroll
+            for (int u = 0; u < AD_DEEP; ++u) a[u].template load<true>(c, b + u * 4 * MT_BLOCK + lane4, 0);
+#pragma unroll
+            for (int u = 0; u < AD_DEEP; ++u) {
+                const uint32_t o = b + u * 4 * MT_BLOCK + lane4;
+                a[u].template step<true>(c, h, s, coef, o, 0, i0 + o);
+            }
+        }
+    } else {
+        const int left = (int)(jb.n - c0);
+#pragma unroll 1
+        for (uint32_t b = wave * MT_BLOCK; (int)b < left; b += 4 * MT_BLOCK) {
+            AdamBlock<PB, GB, S8, NT> a;
+            const uint32_t o = b + lane4;
+            a.template load<false>(c, o, left - (int)o);
+            a.template step<false>(c, h, s, coef, o, left - (int)o, i0 + o);
+        }
     }
 }
 
-template <bool S8>
+template <bool S8, bool NT>
 __global__ __launch_bounds__(256) void multi_adamw_kernel(const MtTable tab, const MtHyper h, const MtClip clip) {
     const MtFind find(tab);
     const float coef = clip_coef(clip);
@@ -418,10 +566,10 @@ __global__ __launch_bounds__(256) void multi_adamw_kernel(const MtTable tab, con
         const float* sc = h.scal + 8 * (size_t)(jb.slot_flags >> 2);
         const MtScal s = {sc[0], sc[1], sc[2], __float_as_uint(sc[3]), __float_as_uint(sc[4])};
         switch (jb.slot_flags & 3) {
-            case 0: adamw_chunk<false, false, S8>(jb, h, s, coef, c0); break;
-            case VAE_MT_GRAD_BF16: adamw_chunk<false, true, S8>(jb, h, s, coef, c0); break;
-            case VAE_MT_PARAM_BF16: adamw_chunk<true, false, S8>(jb, h, s, coef, c0); break;
-            default: adamw_chunk<true, true, S8>(jb, h, s, coef, c0); break;
+            case 0: adamw_chunk<false, false, S8, NT>(jb, h, s, coef, c0); break;
+            case VAE_MT_GRAD_BF16: adamw_chunk<false, true, S8, NT>(jb, h, s, coef, c0); break;
+            case VAE_MT_PARAM_BF16: adamw_chunk<true, false, S8, NT>(jb, h, s, coef, c0); break;
+            default: adamw_chunk<true, true, S8, NT>(jb, h, s, coef, c0); break;
         }
     }
 }
@@ -478,27 +626,24 @@ __global__ __launch_bounds__(256) void moments8_pack_kernel(const float* __restr
     const int lane = threadIdx.x & 63;
     for (long b = (long)blockIdx.x * 4 + (threadIdx.x >> 6); b < nblocks; b += (long)gridDim.x * 4) {
         const size_t k0 = (size_t)b * MT_BLOCK + lane * 4;
-        const float4 a = *(const float4*)(m + k0), c = *(const float4*)(v + k0);
-        const float x[4] = {a.x, a.y, a.z, a.w}, y[4] = {c.x, c.y, c.z, c.w};
-        int bm, bv;
-        block_bases(x, y, bm, bv);
-        const float low = __uint_as_float((uint32_t)(bm + 1) << 20);
-        uint32_t p = 0, q = 0;
+        const float4 x = *(const float4*)(m + k0), y = *(const float4*)(v + k0);
+        AdamBlock<false, false, true, false> a;
+        a.m[0] = x.x; a.m[1] = x.y; a.m[2] = x.z; a.m[3] = x.w;
+        a.v[0] = y.x; a.v[1] = y.y; a.v[2] = y.z; a.v[3] = y.w;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            p |= pack_m(x[k], bm, low, 1u << 19) << 8 * k;
-            q |= pack_v(y[k], bv, 1u << 19) << 8 * k;
-        }
-        *(uint32_t*)(qm + k0) = p;
-        *(uint32_t*)(qv + k0) = q;
-        if (lane == 0) *(uint32_t*)(base + b) = pack_base(bm, bv);
+        for (int k = 0; k < 4; ++k) a.v[k] = fabsf(a.v[k]);      // it has no sign bit
+        const uint32_t bases = a.template pack<true>(0u, 0u, 0u);
+        *(uint32_t*)(qm + k0) = a.qm;
+        *(uint32_t*)(qv + k0) = a.qv;
+        if (lane == 0) *(uint32_t*)(base + b) = bases;
     }
 }
 
 // ---------------------------------------------------------------- host
-static int check_tensors(const char* who, const vae_mt_tensor* t, int count, bool params, long nblocks, int nslots, long* chunks) {
+// *sq_chunks: what the norm's workgroups take in turn, over all tensors
+static int check_tensors(const char* who, const vae_mt_tensor* t, int count, bool params, long nblocks, int nslots, long* sq_chunks) {
     VAE_CHECK(count >= 0 && count <= VAE_MT_MAX_TENSORS && (t || count == 0), "%s: count=%d out of range (0..%d)", who, count, VAE_MT_MAX_TENSORS);
-    long total = 0;
+    long total = 0, sq = 0;
     for (int i = 0; i < count; ++i) {
         VAE_CHECK(t[i].n >= 0 && t[i].n < (1L << 40), "%s: tensor %d has n=%ld", who, i, t[i].n);
         VAE_CHECK((t[i].flags & ~3u) == 0, "%s: tensor %d has unknown flags 0x%x", who, i, t[i].flags);
@@ -512,22 +657,23 @@ static int check_tensors(const char* who, const vae_mt_tensor* t, int count, boo
             VAE_CHECK((long)t[i].slot < nslots, "%s: tensor %d has slot %u of %d", who, i, t[i].slot, nslots);
         }
         total += (t[i].n + MT_CHUNK - 1) / MT_CHUNK;
+        sq += (t[i].n + SQ_CHUNK - 1) / SQ_CHUNK;
     }
     VAE_CHECK(total < 0x7FFFFFFFL, "%s: %ld chunks are too many for one call", who, total);
-    if (chunks) *chunks = total;
+    *sq_chunks = sq;
     return 0;
 }
 
 // the next launch's table, from tensor `at` on; returns the tensor after its last.  Empty tensors keep their slot (their step counts
 // on) but have no chunk: their first chunk is the next tensor's, which find() then prefers.
-static int fill_table(const vae_mt_tensor* t, int count, int at, MtTable& tab) {
+static int fill_table(const vae_mt_tensor* t, int count, int at, int chunk, MtTable& tab) {
     tab.count = 0;
     tab.nchunk = 0;
     for (; at < count && tab.count < MT_TENSORS; ++at) {
         const int k = tab.count++;
         tab.first[k] = tab.nchunk;
         tab.job[k] = {t[at].param, t[at].grad, t[at].n, t[at].block, t[at].slot << 2 | t[at].flags};
-        tab.nchunk += (uint32_t)((t[at].n + MT_CHUNK - 1) / MT_CHUNK);
+        tab.nchunk += (uint32_t)((t[at].n + chunk - 1) / chunk);
     }
     for (int k = tab.count; k < MT_TENSORS; ++k) tab.first[k] = 0xFFFFFFFFu;
     return at;
@@ -542,13 +688,23 @@ static double elem_count(const MtTable& t) {
     for (int k = 0; k < t.count; ++k) n += (double)t.job[k].n;
     return n;
 }
-static int update_grid(uint32_t nchunk) { return nchunk < 2048u ? (int)nchunk : 2048; }
+#ifndef AD_GRID
+#define AD_GRID 1048576u
+#endif
+// bytes a step's launch moves: gradient read, parameter (and remainder) and moments both ways
+static double step_bytes(const MtTable& t, bool eight) {
+    double b = 0;
+    for (int k = 0; k < t.count; ++k)
+        b += (double)t.job[k].n * (((t.job[k].slot_flags & VAE_MT_GRAD_BF16) ? 2 : 4) + 8 + (eight ? 4 : 16));
+    return b;
+}
+static int update_grid(uint32_t nchunk) { return nchunk < AD_GRID ? (int)nchunk : (int)AD_GRID; }
 
 // sum-of-squares launches over a list (with `prep`: the step is prepared by the same launches); adds their partial sums to *np
 static int sumsq_list(const vae_mt_tensor* t, int count, long all_chunks, const MtPrep* prep, bool sums, double* partial, int* np, hipStream_t s) {
     MtTable tab;
     for (int at = 0; at < count;) {
-        at = fill_table(t, count, at, tab);
+        at = fill_table(t, count, at, SQ_CHUNK, tab);
         int n = 0;
         if (sums && tab.nchunk) {
             // of a list longer than one launch each launch gets its share of the partial sums, and at least one
@@ -559,8 +715,8 @@ static int sumsq_list(const vae_mt_tensor* t, int count, long all_chunks, const 
         if (n == 0 && !prep) continue;
         {
             ProfScope prof("multi_sumsq_kernel", 0.0, n ? elem_bytes(tab, 4) : 0.0, s);
-            if (prep) hipLaunchKernelGGL(multi_sumsq_kernel<true>, dim3(n + 1), dim3(256), 0, s, tab, partial + *np, n, *prep);
-            else hipLaunchKernelGGL(multi_sumsq_kernel<false>, dim3(n), dim3(256), 0, s, tab, partial + *np, n, MtPrep{});
+            if (prep) hipLaunchKernelGGL(multi_sumsq_kernel<true>, dim3(n + 1), dim3(SQ_THREADS), 0, s, tab, partial + *np, n, *prep);
+            else hipLaunchKernelGGL(multi_sumsq_kernel<false>, dim3(n), dim3(SQ_THREADS), 0, s, tab, partial + *np, n, MtPrep{});
         }
         VAE_LAUNCH_CHECK("multi_sumsq_kernel");
         *np += n;
@@ -600,7 +756,7 @@ extern "C" int vae_multi_clip(const vae_mt_tensor* tensors, int count, double* p
     if (int rc = sumsq_list(tensors, count, chunks, nullptr, true, partial, &np, s)) return rc;
     MtTable tab;
     for (int at = 0; at < count;) {
-        at = fill_table(tensors, count, at, tab);
+        at = fill_table(tensors, count, at, MT_CHUNK, tab);
         if (!tab.nchunk) continue;
         const MtClip clip = {partial, np, grad_mul, max_norm, norm_out};
         {
@@ -625,6 +781,7 @@ extern "C" int vae_multi_adamw_step(const vae_mt_group* groups, int ngroups, dou
                   sizeof(vae_mt_group));
         VAE_CHECK(q.state_bits == 32 || q.state_bits == 8, "vae_multi_adamw_step: state_bits=%d must be 32 or 8", q.state_bits);
         VAE_CHECK(q.beta1 >= 0.0 && q.beta1 < 1.0 && q.beta2 >= 0.0 && q.beta2 < 1.0, "vae_multi_adamw_step: betas (%g, %g) must be in [0, 1)", q.beta1, q.beta2);
+        VAE_CHECK(q.state_bits == 32 || q.eps >= VAE_MT_MIN_EPS8, "vae_multi_adamw_step: eps=%g: 8-bit moments need at least %g", q.eps, VAE_MT_MIN_EPS8);
         VAE_CHECK(q.eps >= 0.0 && q.weight_decay >= 0.0 && (q.lr_dev || q.lr >= 0.0), "vae_multi_adamw_step: lr=%g, eps=%g and weight_decay=%g must not be negative",
                   q.lr, q.eps, q.weight_decay);
         long chunks = 0;
@@ -648,23 +805,29 @@ extern "C" int vae_multi_adamw_step(const vae_mt_group* groups, int ngroups, dou
         hipLaunchKernelGGL(multi_norm_kernel, dim3(1), dim3(64), 0, s, MtClip{partial, -1, grad_mul, -1.f, norm_out});
         VAE_LAUNCH_CHECK("multi_norm_kernel");
     }
+    // what the step holds in memory, all groups together
+    double bytes = 0.0;
+    for (int k = 0; k < ngroups; ++k)
+        for (int i = 0; i < groups[k].count; ++i) {
+            const vae_mt_tensor& t = groups[k].tensors[i];
+            bytes += (double)t.n * ((t.flags & VAE_MT_GRAD_BF16 ? 2 : 4) + 4 + (groups[k].state_bits == 8 ? 2 : 8));
+        }
     MtTable tab;
     for (int k = 0; k < ngroups; ++k) {
         const vae_mt_group& q = groups[k];
         const MtHyper h = {q.exp_avg, q.exp_avg_sq, (short2*)q.bases, q.remainder, q.scalars, (float)q.beta1, (float)(1.0 - q.beta1), (float)q.beta2,
                            (float)(1.0 - q.beta2), (float)q.eps};
         for (int at = 0; at < q.count;) {
-            at = fill_table(q.tensors, q.count, at, tab);
+            at = fill_table(q.tensors, q.count, at, MT_CHUNK, tab);
             if (!tab.nchunk) continue;
             const MtClip clip = {partial, np, grad_mul, max_norm, norm_out};
             const int grid = update_grid(tab.nchunk);
-            if (q.state_bits == 8) {
-                ProfScope prof("multi_adamw8_kernel", 0.0, elem_bytes(tab, 12) + 4.0 * elem_count(tab), s);
-                hipLaunchKernelGGL(multi_adamw_kernel<true>, dim3(grid), dim3(256), 0, s, tab, h, clip);
-            } else {
-                ProfScope prof("multi_adamw_kernel", 0.0, elem_bytes(tab, 12) + 16.0 * elem_count(tab), s);
-                hipLaunchKernelGGL(multi_adamw_kernel<false>, dim3(grid), dim3(256), 0, s, tab, h, clip);
-            }
+            const bool eight = q.state_bits == 8, nt = bytes > MT_STREAM_BYTES;
+            ProfScope prof(eight ? "multi_adamw8_kernel" : "multi_adamw_kernel", 0.0, step_bytes(tab, eight), s);
+            if (eight && nt) hipLaunchKernelGGL((multi_adamw_kernel<true, true>), dim3(grid), dim3(256), 0, s, tab, h, clip);
+            else if (eight) hipLaunchKernelGGL((multi_adamw_kernel<true, false>), dim3(grid), dim3(256), 0, s, tab, h, clip);
+            else if (nt) hipLaunchKernelGGL((multi_adamw_kernel<false, true>), dim3(grid), dim3(256), 0, s, tab, h, clip);
+            else hipLaunchKernelGGL((multi_adamw_kernel<false, false>), dim3(grid), dim3(256), 0, s, tab, h, clip);
             VAE_LAUNCH_CHECK("multi_adamw_kernel");
         }
     }
@@ -680,7 +843,7 @@ extern "C" int vae_multi_master(const vae_mt_tensor* tensors, int count, const s
     if (check_tensors("vae_multi_master", tensors, count, true, nblocks, 0x7FFFFFFF, &chunks)) return 1;
     MtTable tab;
     for (int at = 0; at < count;) {
-        at = fill_table(tensors, count, at, tab);
+        at = fill_table(tensors, count, at, MT_CHUNK, tab);
         if (!tab.nchunk) continue;
         {
             ProfScope prof("multi_master_kernel", 0.0, 8.0 * elem_count(tab), (hipStream_t)stream);

@@ -287,6 +287,8 @@ class MultiAdamW(torch.optim.Optimizer):
             raise ValueError(f"MultiAdamW: eps={g['eps']} and weight_decay={g['weight_decay']} must not be negative")
         if g["state_bits"] not in (8, 32):
             raise ValueError(f"MultiAdamW: state_bits={g['state_bits']} must be 8 or 32")
+        if g["state_bits"] == 8 and float(g["eps"]) < _lib.MT_MIN_EPS8:
+            raise ValueError(f"MultiAdamW: eps={g['eps']}: 8-bit moments need at least {_lib.MT_MIN_EPS8}")
 
     def add_param_group(self, param_group):
         if len(self._groups) >= _lib.MT_MAX_GROUPS:

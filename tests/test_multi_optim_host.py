@@ -215,3 +215,104 @@ def test_second_moment_decays_where_nearest_would_stand_still():
             q, b = R.pack_tensor(v, t, R.RATE_V, 254, False, nearest=nearest)
         fell = start - R._levels(R.unpack_tensor(q, b, False))[0]
         assert fell.min() >= low and fell.max() <= high, (nearest, fell.min(), fell.max())
+
+
+# ------------------------------------------------------------------------------------------------ the native walk over the lists (on host tensors)
+def step_table(params, layout=None):
+    n = len(params)
+    if layout is None:
+        layout = np.array([[p.numel(), 10 * k, k, int(p.dtype is torch.bfloat16)] for k, p in enumerate(params)], np.int64).reshape(n, 4)
+    jobs = np.zeros(n, optim._JOB)
+    return L.host().collect_step(params, jobs, layout, -1), jobs
+
+
+def test_the_walk_fills_the_table_and_advances_versions():
+    ps = [cpu_param(3, 4), cpu_param(7, dtype=torch.bfloat16), cpu_param(0), cpu_param(())]
+    ps.insert(1, torch.nn.Parameter(torch.zeros(5)))       # without a gradient
+    before = [p._version for p in ps]
+    n, jobs = step_table(ps)
+    have = [k for k, p in enumerate(ps) if p.grad is not None]
+    assert n == 4 and [p._version - b for p, b in zip(ps, before)] == [1, 0, 1, 1, 1]
+    for row, k in zip(jobs, have):
+        p = ps[k]
+        assert (row["param"], row["grad"], row["n"], row["block"], row["slot"]) == (p.data_ptr(), p.grad.data_ptr(), p.numel(), 10 * k, k)
+        assert row["flags"] == (3 if p.dtype is torch.bfloat16 else 0) and row["reserved"] == 0
+    table = np.zeros(5, optim._JOB)
+    assert L.host().collect_grads(ps, table, -1, False) == 4
+    assert list(table["grad"][:4]) == list(jobs["grad"][:4]) and list(table["flags"][:4]) == [0, 2, 0, 0] and list(table["n"][:4]) == [12, 7, 0, 1]
+
+
+def test_the_walk_over_all_parameters_reads_only():
+    ps = [cpu_param(3, 4), torch.nn.Parameter(torch.zeros(5)), cpu_param(7, dtype=torch.bfloat16)]
+    layout = np.array([[12, 0, 0, 0], [5, 1, 1, 0], [7, 2, 2, 1]], np.int64)
+    jobs, before = np.zeros(3, optim._JOB), [p._version for p in ps]
+    assert L.host().collect_params(ps, jobs, layout, -1) == 3 and [p._version for p in ps] == before
+    assert list(jobs["param"]) == [p.data_ptr() for p in ps] and list(jobs["flags"]) == [0, 0, 3] and list(jobs["block"]) == [0, 1, 2]
+    assert L.host().collect_params([ps[0], strided()], jobs, np.array([[12, 0, 0, 0], [24, 1, 1, 0]], np.int64), -1) == -1
+
+
+def test_the_walk_leaves_everything_else_to_the_general_way():
+    def one(p, **kw):
+        row = dict(n=p.numel(), flags=int(p.dtype is torch.bfloat16))
+        row.update(kw)
+        before = p._version
+        n, _ = step_table([cpu_param(2), p], np.array([[2, 0, 0, 0], [row["n"], 1, 1, row["flags"]]], np.int64))
+        assert n == -1 and p._version == before
+    p = cpu_param(4, 6)
+    one(p, n=23)                                             # another size than the state was made for
+    one(p, flags=1)                                          # another type
+    one(strided())
+    q = cpu_param(4, 6)
+    q.grad = torch.zeros(6, 4).t()
+    one(q)                                                   # the gradient in another order
+    q.grad = torch.zeros(1, 1).expand(4, 6)
+    one(q)
+    h = cpu_param(4, dtype=torch.float16)
+    one(h)
+    s = torch.nn.Parameter(torch.zeros(3, 3))
+    s.grad = torch.eye(3).to_sparse()
+    one(s)
+    c = cpu_param(4)
+    assert L.host().collect_step([c], np.zeros(1, optim._JOB), np.array([[4, 0, 0, 0]], np.int64), 0) == -1       # not on that GPU
+    assert L.host().collect_step(["no tensor"], np.zeros(1, optim._JOB), np.zeros((1, 4), np.int64), -1) == -1
+    assert L.host().collect_step([], np.zeros(0, optim._JOB), np.zeros((0, 4), np.int64), -1) == 0
+
+
+def strided():
+    p = torch.nn.Parameter(torch.zeros(6, 4).t())
+    p.grad = torch.zeros(6, 4).t()
+    return p
+
+
+def test_the_walk_finds_gradients_that_overlap():
+    flat = torch.zeros(20)
+    ps = [torch.nn.Parameter(torch.zeros(8)) for _ in range(2)]
+    for shift, ok in ((8, True), (7, False), (0, False)):
+        ps[0].grad, ps[1].grad = flat[:8], flat[shift:shift + 8]
+        before = flat._version
+        n = L.host().collect_grads(ps, np.zeros(2, optim._JOB), -1, True)
+        assert n == (2 if ok else -1) and (flat._version > before) == ok
+        assert L.host().collect_grads(ps, np.zeros(2, optim._JOB), -1, False) == 2       # reading them is no matter
+
+
+def test_the_walk_refuses_tables_that_are_too_short():
+    ps = [cpu_param(2), cpu_param(2)]
+    with pytest.raises(ValueError, match="shorter"):
+        L.host().collect_step(ps, np.zeros(1, optim._JOB), np.zeros((2, 4), np.int64), -1)
+    with pytest.raises(ValueError, match="shorter"):
+        L.host().collect_step(ps, np.zeros(2, optim._JOB), np.zeros((1, 4), np.int64), -1)
+    with pytest.raises(ValueError, match="shorter"):
+        L.host().collect_grads(ps, np.zeros(1, optim._JOB), -1, False)
+    with pytest.raises((TypeError, BufferError, ValueError)):
+        L.host().collect_grads(ps, 7, -1, False)
+
+
+def test_the_extension_is_refused_under_another_torch(monkeypatch):
+    L.host()
+    monkeypatch.setattr(L, "_host", None)
+    monkeypatch.setattr(torch, "__version__", "1.0.0")
+    with pytest.raises(RuntimeError, match="rebuild"):
+        L.host()
+    monkeypatch.setattr(L, "HOST_PATH", "/nowhere/_host.so")
+    with pytest.raises(RuntimeError, match="not found"):
+        L.host()

@@ -79,57 +79,51 @@ def _dense(t):
     return True
 
 
-def _collect_grads(params, who):
-    """(tensors, their gradients) of the parameters that have one, and the gradients' addresses, lengths and types"""
-    grads = []
-    for p in params:
-        g = p.grad
-        if g is None:
-            continue
+def _grad_jobs(parameters, who, write):
+    """(table of the parameters' gradients, their number, one of them or None).  ``write``: they are written in place"""
+    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    first = next((p.grad for p in params if p.grad is not None), None)
+    if first is None:
+        return None, 0, None
+    _lib.check_device(first)
+    jobs = np.empty(len(params), _JOB)
+    n = _lib.host().collect_grads(params, jobs, first.get_device(), write)
+    if n >= 0:
+        return jobs, n, first
+    grads = [p.grad for p in params if p.grad is not None]
+    for g in grads:
         if g.layout is not torch.strided or g.dtype not in _TYPES:
             raise TypeError(f"{who}: a gradient is {g.layout} {g.dtype}; dense fp32 and bf16 gradients are supported")
-        if not _dense(g):
-            raise ValueError(f"{who}: a gradient of shape {tuple(g.shape)} with strides {g.stride()} has gaps or overlaps and cannot be written "
-                             "in place")
-        grads.append(g)
-    return grads
-
-
-def _norm_jobs(grads, who):
-    jobs = np.zeros(max(len(grads), 1), _JOB)
-    if grads:
-        dev = grads[0].get_device()
-        if any(g.get_device() != dev for g in grads):
-            raise RuntimeError(f"{who}: the gradients live on several devices")
-        _lib.check_device(grads[0])
-        k = len(grads)
-        jobs["grad"][:k] = [g.data_ptr() for g in grads]
-        jobs["n"][:k] = [g.numel() for g in grads]
-        jobs["flags"][:k] = [_lib.MT_GRAD_BF16 if g.dtype is torch.bfloat16 else 0 for g in grads]
-    return jobs
-
-
-def _as_list(parameters):
-    return [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-
-
-def _refuse_duplicates(grads, who):
-    if len({g.data_ptr() for g in grads if g.numel()}) != sum(g.numel() > 0 for g in grads):
-        raise ValueError(f"{who}: two of the gradients are the same memory")
+        if g.device != first.device:
+            raise RuntimeError(f"{who}: the gradients live on {first.device} and {g.device}")
+    if write:
+        for g in grads:
+            if not _dense(g):
+                raise ValueError(f"{who}: a gradient of shape {tuple(g.shape)} with strides {g.stride()} has gaps or overlaps and cannot be written "
+                                 "in place")
+        spans = sorted((g.data_ptr(), g.data_ptr() + g.nbytes) for g in grads if g.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError(f"{who}: two of the gradients are the same memory, wholly or in part")
+        increment_version(grads)
+    else:
+        grads = [g if _dense(g) else g.contiguous() for g in grads]
+    jobs["grad"][:len(grads)] = [g.data_ptr() for g in grads]
+    jobs["n"][:len(grads)] = [g.numel() for g in grads]
+    jobs["flags"][:len(grads)] = [_lib.MT_GRAD_BF16 if g.dtype is torch.bfloat16 else 0 for g in grads]
+    return jobs, len(grads), grads
 
 
 @torch.no_grad()
 def grad_norm(parameters):
     """Global L2 norm of the parameters' gradients as a 0-dim fp32 tensor: one launch per 192 tensors and one that finishes the
     sum.  Squares and sums in 64 bits, in a fixed order."""
-    grads = _collect_grads(_as_list(parameters), "grad_norm")
-    if not grads:
+    jobs, n, keep = _grad_jobs(parameters, "grad_norm", False)
+    if n == 0:
         return torch.zeros(())
-    jobs = _norm_jobs(grads, "grad_norm")
-    dev = grads[0].device
-    partial = torch.empty(_lib.call("vae_multi_partials", len(grads)), dtype=torch.float64, device=dev)
+    dev = torch.device("cuda", torch.cuda.current_device())
+    partial = torch.empty(_lib.call("vae_multi_partials", n), dtype=torch.float64, device=dev)
     out = torch.empty((), device=dev)
-    _lib.call("vae_multi_grad_norm", jobs.ctypes.data, len(grads), partial.data_ptr(), 1.0, out.data_ptr(), _lib.current_stream())
+    _lib.call("vae_multi_grad_norm", jobs.ctypes.data, n, partial.data_ptr(), 1.0, out.data_ptr(), _lib.current_stream())
     return out
 
 
@@ -143,21 +137,18 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
         raise ValueError(f"clip_grad_norm_: max_norm={max_norm} must not be negative or NaN")
     if float(norm_type) != 2.0:
         raise ValueError(f"clip_grad_norm_: norm_type={norm_type}; only the L2 norm is computed")
-    params = _as_list(parameters)
-    grads = _collect_grads(params, "clip_grad_norm_")
-    if not grads:
-        return torch.zeros(())
-    _refuse_duplicates(grads, "clip_grad_norm_")
     if error_if_nonfinite:
-        norm = grad_norm(params)
+        parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+        norm = grad_norm(parameters)
         if not bool(torch.isfinite(norm)):
             raise RuntimeError(f"clip_grad_norm_: the gradients' norm is {norm.item()}, so it cannot be clipped")
-    jobs = _norm_jobs(grads, "clip_grad_norm_")
-    dev = grads[0].device
-    partial = torch.empty(_lib.call("vae_multi_partials", len(grads)), dtype=torch.float64, device=dev)
+    jobs, n, keep = _grad_jobs(parameters, "clip_grad_norm_", True)
+    if n == 0:
+        return torch.zeros(())
+    dev = torch.device("cuda", torch.cuda.current_device())
+    partial = torch.empty(_lib.call("vae_multi_partials", n), dtype=torch.float64, device=dev)
     out = torch.empty((), device=dev)
-    _lib.call("vae_multi_clip", jobs.ctypes.data, len(grads), partial.data_ptr(), 1.0, max_norm, out.data_ptr(), _lib.current_stream())
-    increment_version(grads)
+    _lib.call("vae_multi_clip", jobs.ctypes.data, n, partial.data_ptr(), 1.0, max_norm, out.data_ptr(), _lib.current_stream())
     return out
 
 
@@ -189,8 +180,9 @@ class _GroupState:
         self.steps = z(len(params), dtype=torch.int64)
         self.scalars = z(len(params), 8)
         self.jobs = np.zeros(len(params), _JOB)
-        self.jobs["n"], self.jobs["block"], self.jobs["slot"] = self.n, self.start, np.arange(len(params))
+        self.index = self.device.index
         self.param_flags = [_lib.MT_PARAM_BF16 if d is torch.bfloat16 else 0 for d in self.dtypes]
+        self.layout = np.stack([self.n, self.start, np.arange(len(params)), self.param_flags], 1).astype(np.int64)
         self.c = _lib.MtGroup(state_bits=state_bits, nslots=len(params), exp_avg=self.exp_avg.data_ptr(),
                               exp_avg_sq=self.exp_avg_sq.data_ptr(), bases=_lib.ptr(self.bases), remainder=_lib.ptr(self.remainder),
                               nblocks=self.nblocks, steps=self.steps.data_ptr(), scalars=self.scalars.data_ptr())
@@ -208,8 +200,11 @@ class _GroupState:
         return p
 
     def collect(self):
-        """fills the table of the tensors that have a gradient; returns (their number, the tensors to keep until the launch, the
-        parameters that will be written)"""
+        """fills the table of the tensors that have a gradient; returns their number and what has to live until the launch"""
+        n = _lib.host().collect_step(self.params, self.jobs, self.layout, self.index)
+        if n >= 0:
+            self.c.tensors, self.c.count = self.jobs.ctypes.data, n
+            return n, None
         ptrs, gptrs, flags, keep, live, at = [], [], [], [], [], []
         for k, p in enumerate(self.params):
             g = p.grad
@@ -230,11 +225,13 @@ class _GroupState:
             live.append(p)
             at.append(k)
         n = len(live)
-        jobs = self.jobs if n == len(self.params) else self.jobs[at]
-        jobs["param"], jobs["grad"], jobs["flags"] = ptrs, gptrs, flags
+        jobs = np.zeros(max(n, 1), _JOB)
+        jobs["param"][:n], jobs["grad"][:n], jobs["flags"][:n] = ptrs, gptrs, flags
+        jobs["n"][:n], jobs["block"][:n], jobs["slot"][:n] = self.layout[at, 0], self.layout[at, 1], self.layout[at, 2]
         keep.append(jobs)
         self.c.tensors, self.c.count = jobs.ctypes.data, n
-        return n, keep, live
+        increment_version(live)      # written through their addresses: whoever watches the version counters has to see it
+        return n, keep
 
     def view(self, flat, k):
         """element run k of a buffer in the state's layout, in the parameter's shape"""
@@ -362,17 +359,16 @@ class MultiAdamW(torch.optim.Optimizer):
         if max_norm is not None and not clip >= 0.0:
             raise ValueError(f"MultiAdamW: max_norm={max_norm} must not be negative or NaN")
         _lib.check_device(self.grad_norm)
-        keep, live, total = [], [], 0
+        keep, total = [], 0
         for k, (g, st) in enumerate(zip(self.param_groups, self._groups)):
             if len(g["params"]) != len(st.params):
                 raise RuntimeError("MultiAdamW: a param group's list of tensors was changed")
             self._check_group(g)
             if g["state_bits"] != st.bits:
                 raise RuntimeError(f"MultiAdamW: state_bits of a group was changed from {st.bits} to {g['state_bits']}")
-            n, kept, written = st.collect()
+            n, kept = st.collect()
             total += n
             keep.append(kept)
-            live += written
             c, lr = st.c, g["lr"]
             c.lr, c.lr_dev = (0.0, lr.data_ptr()) if isinstance(lr, torch.Tensor) else (float(lr), None)
             (c.beta1, c.beta2), c.eps, c.weight_decay = g["betas"], g["eps"], g["weight_decay"]
@@ -389,7 +385,6 @@ class MultiAdamW(torch.optim.Optimizer):
             self.grad_norm.record_stream(cur)
         _lib.call("vae_multi_adamw_step", ctypes.byref(self._c), len(self._groups), self._partial.data_ptr(), float(self.grad_mul), clip,
                   self.grad_norm.data_ptr() if clip >= 0.0 else None, stream)
-        increment_version(live)      # written through their addresses: whoever watches the version counters has to see it
 
     # -------------------------------------------------------------------------------- state
     def flat_moments(self, group=0):
@@ -414,12 +409,14 @@ class MultiAdamW(torch.optim.Optimizer):
         st = self._groups[group]
         _lib.check_device(st.exp_avg)
         out = torch.zeros(max(st.nblocks, 1) * _lib.MT_BLOCK, device=st.device)
-        jobs = st.jobs.copy()
-        for k in range(len(st.params)):
-            st.check_param(k)
-        jobs["param"] = [p.data_ptr() for p in st.params]
-        jobs["grad"] = jobs["param"]       # not read
-        jobs["flags"] = [f * (_lib.MT_PARAM_BF16 | _lib.MT_GRAD_BF16) for f in st.param_flags]
+        jobs = np.zeros(len(st.params), _JOB)
+        if _lib.host().collect_params(st.params, jobs, st.layout, st.index) < 0:
+            for k in range(len(st.params)):
+                st.check_param(k)
+            jobs["n"], jobs["block"], jobs["slot"] = st.layout[:, 0], st.layout[:, 1], st.layout[:, 2]
+            jobs["param"] = [p.data_ptr() for p in st.params]
+            jobs["grad"] = jobs["param"]       # not read
+            jobs["flags"] = [f * (_lib.MT_PARAM_BF16 | _lib.MT_GRAD_BF16) for f in st.param_flags]
         _lib.call("vae_multi_master", jobs.ctypes.data, len(st.params), _lib.ptr(st.remainder), out.data_ptr(), st.nblocks, _lib.current_stream())
         return out
 
@@ -479,9 +476,9 @@ class MultiAdamW(torch.optim.Optimizer):
             st.steps.copy_(torch.tensor([int(e.get("step", 0)) for e in row], dtype=torch.int64))
             if st.remainder is not None:
                 st.remainder.zero_()
-                for k, e in enumerate(row):
-                    if "remainder" in e:
-                        st.view(st.remainder, k).copy_(e["remainder"].view(st.shapes[k]))
+                have = [k for k, e in enumerate(row) if "remainder" in e and st.dtypes[k] is torch.bfloat16]
+                if have:
+                    torch._foreach_copy_([st.view(st.remainder, k) for k in have], [row[k]["remainder"].view(st.shapes[k]) for k in have])
             self._load_moments(st, row)
 
     @staticmethod
@@ -511,36 +508,33 @@ class MultiAdamW(torch.optim.Optimizer):
 
     def _load_moments(self, st, row):
         _lib.check_device(st.exp_avg)
-        eight = any("exp_avg_q" in e for e in row)
-        full = any("exp_avg" in e for e in row)
-        q = st if st.bits == 8 else None
-        if st.bits == 32:
-            m, v = st.exp_avg, st.exp_avg_sq
-            m.zero_(), v.zero_()
-        elif full:
-            m, v = torch.zeros_like(st.exp_avg, dtype=torch.float32), torch.zeros_like(st.exp_avg, dtype=torch.float32)
-        if eight or st.bits == 8:
-            qm, qv = (st.exp_avg, st.exp_avg_sq) if q else (torch.zeros_like(m, dtype=torch.uint8), torch.zeros_like(m, dtype=torch.uint8))
-            bases = st.bases if q else torch.zeros(max(st.nblocks, 1), 2, dtype=torch.int16, device=st.device)
-            qm.zero_(), qv.zero_(), bases.zero_()
-        if st.bits == 8 and full:
-            for k, e in enumerate(row):
-                if "exp_avg" in e:
-                    st.view(m, k).copy_(e["exp_avg"])
-                    st.view(v, k).copy_(e["exp_avg_sq"])
-            _lib.call("vae_moments8_pack", m.data_ptr(), v.data_ptr(), qm.data_ptr(), qv.data_ptr(), bases.data_ptr(), bases.shape[0],
-                      _lib.current_stream())
+        eight, full = [k for k, e in enumerate(row) if "exp_avg_q" in e], [k for k, e in enumerate(row) if "exp_avg" in e]
+        scratch = lambda dtype: (torch.zeros_like(st.exp_avg, dtype=dtype), torch.zeros_like(st.exp_avg, dtype=dtype))  # noqa: E731
+
+        def fill(dst, view, which, keys):
+            if which:
+                for buf, key in zip(dst, keys):
+                    torch._foreach_copy_([view(buf, k) for k in which], [row[k][key] for k in which])
+        if st.bits == 8:
+            q, bases = (st.exp_avg, st.exp_avg_sq), st.bases
+            if full:
+                f32 = scratch(torch.float32)
+                fill(f32, st.view, full, ("exp_avg", "exp_avg_sq"))
+                _lib.call("vae_moments8_pack", f32[0].data_ptr(), f32[1].data_ptr(), q[0].data_ptr(), q[1].data_ptr(), bases.data_ptr(),
+                          bases.shape[0], _lib.current_stream())
+            else:
+                q[0].zero_(), q[1].zero_(), bases.zero_()
+        elif eight:
+            q, bases = scratch(torch.uint8), torch.zeros(max(st.nblocks, 1), 2, dtype=torch.int16, device=st.device)
         if eight:
-            for k, e in enumerate(row):
-                if "exp_avg_q" in e:
-                    st.run(qm, k).copy_(e["exp_avg_q"].reshape(-1))
-                    st.run(qv, k).copy_(e["exp_avg_sq_q"].reshape(-1))
-                    bases[st.rows(k), 0] = e["exp_avg_base"].reshape(-1).to(device=st.device, dtype=torch.int16)
-                    bases[st.rows(k), 1] = e["exp_avg_sq_base"].reshape(-1).to(device=st.device, dtype=torch.int16)
+            fill(q, st.run, eight, ("exp_avg_q", "exp_avg_sq_q"))
+            rows = torch.cat([torch.arange(st.rows(k).start, st.rows(k).stop) for k in eight]).to(st.device)
+            for j, key in enumerate(("exp_avg_base", "exp_avg_sq_base")):
+                bases[rows, j] = torch.cat([row[k][key].reshape(-1) for k in eight]).to(device=st.device, dtype=torch.int16)
         if st.bits == 32:
+            m = (st.exp_avg, st.exp_avg_sq)
             if eight:
-                self._unpack(st, qm, qv, bases, m, v)
-            for k, e in enumerate(row):
-                if "exp_avg" in e:
-                    st.view(m, k).copy_(e["exp_avg"])
-                    st.view(v, k).copy_(e["exp_avg_sq"])
+                self._unpack(st, q[0], q[1], bases, *m)
+            else:
+                m[0].zero_(), m[1].zero_()
+            fill(m, st.view, full, ("exp_avg", "exp_avg_sq"))

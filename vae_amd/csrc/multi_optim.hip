@@ -315,7 +315,8 @@ __device__ __forceinline__ void scale_chunk(void* g, long c0, long n, float coef
 __global__ __launch_bounds__(256) void multi_scale_kernel(const MtTable tab, const MtClip clip) {
     const MtFind find(tab);
     const float coef = clip_coef(clip);
-    for (uint32_t c = blockIdx.x; c < tab.nchunk; c += gridDim.x) {
+    for (uint32_t w = blockIdx.x; w < tab.nchunk; w += gridDim.x) {
+        const uint32_t c = tab.nchunk - 1 - w;      // what the norm has read last is still in the caches
         const int j = find(c);
         const MtJob& jb = tab.job[j];
         const long c0 = (long)(c - tab.first[j]) * MT_CHUNK;
@@ -559,7 +560,8 @@ template <bool S8, bool NT>
 __global__ __launch_bounds__(256) void multi_adamw_kernel(const MtTable tab, const MtHyper h, const MtClip clip) {
     const MtFind find(tab);
     const float coef = clip_coef(clip);
-    for (uint32_t c = blockIdx.x; c < tab.nchunk; c += gridDim.x) {
+    for (uint32_t w = blockIdx.x; w < tab.nchunk; w += gridDim.x) {
+        const uint32_t c = tab.nchunk - 1 - w;      // what the norm has read last is still in the caches
         const int j = find(c);
         const MtJob& jb = tab.job[j];
         const long c0 = (long)(c - tab.first[j]) * MT_CHUNK;
@@ -575,47 +577,71 @@ __global__ __launch_bounds__(256) void multi_adamw_kernel(const MtTable tab, con
 }
 
 // masters of the bf16 parameters (and the fp32 parameters themselves) in the state's layout, padding 0
+template <bool PB, bool FULL>
+__device__ __forceinline__ void master_chunk(const MtChunk& c, float* out, int left) {
+    float w[MT_CHUNK / 1024][4];
+    short4v r[MT_CHUNK / 1024];
+    u16x4u p[MT_CHUNK / 1024];
+#pragma unroll
+    for (int u = 0; u < MT_CHUNK / 1024; ++u) {
+        const uint32_t o = (u * 256 + threadIdx.x) * 4u;
+        if (!FULL && (int)(o & ~(MT_BLOCK - 1u)) >= left) break;       // a block behind the tensor's last is another tensor's
+        if (PB) {
+            load4<FULL>((const bf16_t*)c.p, o, left - (int)o, p[u]);
+            r[u] = *(const short4v*)(c.rem + o);
+        } else {
+            load4<FULL>((const float*)c.p, o, left - (int)o, w[u]);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < MT_CHUNK / 1024; ++u) {
+        const uint32_t o = (u * 256 + threadIdx.x) * 4u;
+        if (!FULL && (int)(o & ~(MT_BLOCK - 1u)) >= left) break;
+        if (PB) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[u][k] = FULL || (int)o + k < left ? join_master(p[u][k], r[u][k]) : 0.f;
+        }
+        *(f32x4*)(out + o) = f32x4{w[u][0], w[u][1], w[u][2], w[u][3]};
+    }
+}
 __global__ __launch_bounds__(256) void multi_master_kernel(const MtTable tab, const short* __restrict__ rem, float* __restrict__ out) {
     const MtFind find(tab);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (uint32_t c = blockIdx.x; c < tab.nchunk; c += gridDim.x) {
         const int j = find(c);
         const MtJob& jb = tab.job[j];
         const long c0 = (long)(c - tab.first[j]) * MT_CHUNK;
-        for (int u = 0; u < MT_CHUNK / MT_BLOCK / 4; ++u) {
-            const long b0 = c0 + (u * 4 + wave) * MT_BLOCK, i = b0 + lane * 4;
-            if (b0 >= jb.n) break;
-            const size_t k0 = ((size_t)jb.block + b0 / MT_BLOCK) * MT_BLOCK + lane * 4;
-            f32x4 w = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (i + k < jb.n)
-                    w[k] = (jb.slot_flags & VAE_MT_PARAM_BF16) ? join_master(((const bf16_t*)jb.p)[i + k], rem[k0 + k]) : ((const float*)jb.p)[i + k];
-            *(f32x4*)(out + k0) = w;
-        }
+        const size_t k0 = (size_t)jb.block * MT_BLOCK + c0;
+        const bool bf = jb.slot_flags & VAE_MT_PARAM_BF16, full = jb.n - c0 >= MT_CHUNK;
+        const int left = full ? MT_CHUNK : (int)(jb.n - c0);
+        MtChunk k = {(char*)jb.p + c0 * (bf ? 2 : 4), nullptr, nullptr, nullptr, (short*)rem + k0, nullptr};
+        if (bf && full) master_chunk<true, true>(k, out + k0, left);
+        else if (bf) master_chunk<true, false>(k, out + k0, left);
+        else if (full) master_chunk<false, true>(k, out + k0, left);
+        else master_chunk<false, false>(k, out + k0, left);
     }
 }
 
+// 8 elements a thread: 16-byte stores
 template <bool BF>
 __global__ __launch_bounds__(256) void moments8_unpack_kernel(const uint8_t* __restrict__ qm, const uint8_t* __restrict__ qv,
-                                                              const short2* __restrict__ base, void* __restrict__ m, void* __restrict__ v, long nblocks) {
-    const int lane = threadIdx.x & 63;
-    for (long b = (long)blockIdx.x * 4 + (threadIdx.x >> 6); b < nblocks; b += (long)gridDim.x * 4) {
-        const size_t k0 = (size_t)b * MT_BLOCK + lane * 4;
-        const uint32_t a = *(const uint32_t*)(qm + k0), c = *(const uint32_t*)(qv + k0);
-        const short2 bs = base[b];
-        float x[4], y[4];
+                                                              const short2* __restrict__ base, void* __restrict__ m, void* __restrict__ v, long n) {
+    for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (long)gridDim.x * 2048) {
+        const uint2 a = *(const uint2*)(qm + i), c = *(const uint2*)(qv + i);
+        const short2 b = base[i / MT_BLOCK];
+        float x[8], y[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            x[k] = unpack_m((a >> 8 * k) & 255u, bs.x);
-            y[k] = unpack_v((c >> 8 * k) & 255u, bs.y);
+        for (int k = 0; k < 8; ++k) {
+            x[k] = unpack_m(((k < 4 ? a.x : a.y) >> 8 * (k & 3)) & 255u, b.x);
+            y[k] = unpack_v(((k < 4 ? c.x : c.y) >> 8 * (k & 3)) & 255u, b.y);
         }
         if (BF) {      // 4 significant bits: exact
-            *(uint2*)((bf16_t*)m + k0) = make_uint2(pack2bf(x[0], x[1]), pack2bf(x[2], x[3]));
-            *(uint2*)((bf16_t*)v + k0) = make_uint2(pack2bf(y[0], y[1]), pack2bf(y[2], y[3]));
+            *(uint4*)((bf16_t*)m + i) = make_uint4(pack2bf(x[0], x[1]), pack2bf(x[2], x[3]), pack2bf(x[4], x[5]), pack2bf(x[6], x[7]));
+            *(uint4*)((bf16_t*)v + i) = make_uint4(pack2bf(y[0], y[1]), pack2bf(y[2], y[3]), pack2bf(y[4], y[5]), pack2bf(y[6], y[7]));
         } else {
-            *(float4*)((float*)m + k0) = make_float4(x[0], x[1], x[2], x[3]);
-            *(float4*)((float*)v + k0) = make_float4(y[0], y[1], y[2], y[3]);
+            *(float4*)((float*)m + i) = make_float4(x[0], x[1], x[2], x[3]);
+            *(float4*)((float*)m + i + 4) = make_float4(x[4], x[5], x[6], x[7]);
+            *(float4*)((float*)v + i) = make_float4(y[0], y[1], y[2], y[3]);
+            *(float4*)((float*)v + i + 4) = make_float4(y[4], y[5], y[6], y[7]);
         }
     }
 }
@@ -854,9 +880,10 @@ extern "C" int vae_multi_master(const vae_mt_tensor* tensors, int count, const s
     return 0;
 }
 
-static int blocks_grid(long nblocks) {
-    const long g = (nblocks + 3) / 4;
-    return (int)(g < 4096 ? g : 4096);
+// workgroups of four blocks (pack) or eight (unpack) each
+static int blocks_grid(long nblocks, int per) {
+    const long g = (nblocks + per - 1) / per;
+    return (int)(g < (1 << 20) ? g : 1 << 20);
 }
 
 extern "C" int vae_moments8_unpack(const void* exp_avg_q, const void* exp_avg_sq_q, const short* bases, void* exp_avg, void* exp_avg_sq, long nblocks,
@@ -869,11 +896,11 @@ extern "C" int vae_moments8_unpack(const void* exp_avg_q, const void* exp_avg_sq
     {
         ProfScope prof("moments8_unpack_kernel", 0.0, 256.0 * nblocks * (bf16_out ? 6 : 10), (hipStream_t)stream);
         if (bf16_out)
-            hipLaunchKernelGGL(moments8_unpack_kernel<true>, dim3(blocks_grid(nblocks)), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)exp_avg_q,
-                               (const uint8_t*)exp_avg_sq_q, (const short2*)bases, exp_avg, exp_avg_sq, nblocks);
+            hipLaunchKernelGGL(moments8_unpack_kernel<true>, dim3(blocks_grid(nblocks, 8)), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)exp_avg_q,
+                               (const uint8_t*)exp_avg_sq_q, (const short2*)bases, exp_avg, exp_avg_sq, nblocks * MT_BLOCK);
         else
-            hipLaunchKernelGGL(moments8_unpack_kernel<false>, dim3(blocks_grid(nblocks)), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)exp_avg_q,
-                               (const uint8_t*)exp_avg_sq_q, (const short2*)bases, exp_avg, exp_avg_sq, nblocks);
+            hipLaunchKernelGGL(moments8_unpack_kernel<false>, dim3(blocks_grid(nblocks, 8)), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)exp_avg_q,
+                               (const uint8_t*)exp_avg_sq_q, (const short2*)bases, exp_avg, exp_avg_sq, nblocks * MT_BLOCK);
     }
     VAE_LAUNCH_CHECK("moments8_unpack_kernel");
     return 0;
@@ -887,7 +914,7 @@ extern "C" int vae_moments8_pack(const float* exp_avg, const float* exp_avg_sq, 
               "vae_moments8_pack: buffers must be 16-byte aligned");
     {
         ProfScope prof("moments8_pack_kernel", 0.0, 256.0 * nblocks * 10, (hipStream_t)stream);
-        hipLaunchKernelGGL(moments8_pack_kernel, dim3(blocks_grid(nblocks)), dim3(256), 0, (hipStream_t)stream, exp_avg, exp_avg_sq, (uint8_t*)exp_avg_q,
+        hipLaunchKernelGGL(moments8_pack_kernel, dim3(blocks_grid(nblocks, 4)), dim3(256), 0, (hipStream_t)stream, exp_avg, exp_avg_sq, (uint8_t*)exp_avg_q,
                            (uint8_t*)exp_avg_sq_q, (short2*)bases, nblocks);
     }
     VAE_LAUNCH_CHECK("moments8_pack_kernel");

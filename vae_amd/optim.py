@@ -217,7 +217,8 @@ class _GroupState:
                 raise RuntimeError(f"MultiAdamW: the gradient of parameter {k} is {tuple(g.shape)} on {g.device}, the parameter "
                                    f"{self.shapes[k]} on {self.device}")
             if not (g.is_contiguous() if self.contiguous[k] else g.stride() == self.strides[k]):
-                g = torch.empty_like(p, dtype=g.dtype).copy_(g)       # into the parameter's order of elements
+                with torch.no_grad():
+                    g = torch.empty_like(p, dtype=g.dtype).copy_(g)       # into the parameter's order of elements
                 keep.append(g)
             ptrs.append(p.data_ptr())
             gptrs.append(g.data_ptr())
@@ -338,18 +339,19 @@ class MultiAdamW(torch.optim.Optimizer):
     def step(self, closure=None, max_norm=None):
         """One step; with ``max_norm`` the gradients' global norm (over all groups) is clipped to it first.  ``closure``, as in torch,
         recomputes the loss and its gradients; its value is returned."""
-        for hook in (*_global_pre_hooks.values(), *self._optimizer_step_pre_hooks.values()):
-            changed = hook(self, (closure,), {"max_norm": max_norm})
-            if changed is not None:
-                (closure,), max_norm = changed[0], changed[1].get("max_norm")
+        if _global_pre_hooks or self._optimizer_step_pre_hooks:
+            for hook in (*_global_pre_hooks.values(), *self._optimizer_step_pre_hooks.values()):
+                changed = hook(self, (closure,), {"max_norm": max_norm})
+                if changed is not None:
+                    (closure,), max_norm = changed[0], changed[1].get("max_norm")
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        with torch.no_grad():
-            self._step(max_norm)
-        for hook in (*self._optimizer_step_post_hooks.values(), *_global_post_hooks.values()):
-            hook(self, (closure,), {"max_norm": max_norm})
+        self._step(max_norm)
+        if _global_post_hooks or self._optimizer_step_post_hooks:
+            for hook in (*self._optimizer_step_post_hooks.values(), *_global_post_hooks.values()):
+                hook(self, (closure,), {"max_norm": max_norm})
         return loss
 
     step.hooked = True      # torch would wrap it into a profiler range, 14 us of host time a step
@@ -408,7 +410,8 @@ class MultiAdamW(torch.optim.Optimizer):
         """32-bit values of a group's parameters in the state's layout: a bf16 parameter's master, an fp32 parameter itself"""
         st = self._groups[group]
         _lib.check_device(st.exp_avg)
-        out = torch.zeros(max(st.nblocks, 1) * _lib.MT_BLOCK, device=st.device)
+        # every block is some tensor's and is written whole
+        out = (torch.empty if st.nblocks else torch.zeros)(max(st.nblocks, 1) * _lib.MT_BLOCK, device=st.device)
         jobs = np.zeros(len(st.params), _JOB)
         if _lib.host().collect_params(st.params, jobs, st.layout, st.index) < 0:
             for k in range(len(st.params)):

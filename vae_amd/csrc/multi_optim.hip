@@ -44,12 +44,13 @@ namespace vae {
 #define SQ_DEEP 4                // 16-byte loads a thread of the norm has in flight
 #define SQ_CHUNK (SQ_THREADS * SQ_DEEP * 4)
 
-// The moments and remainders of a step whose tensors and state are larger than this are loaded and stored past the caches: the last
-// level holds 256 MB, what is larger is gone before the next step reads it.  69.8 M parameters (1.1 GB): 347 us against 377, with
-// 8-bit moments (0.7 GB) 188 against 208; 4.1 M parameters (65 MB), which do stay: 26 us against 22.  Parameters and gradients stay
-// cached in any case: the norm has just read the gradients, the next forward pass reads the parameters (bf16, 20 M of
-// them: 96 us against 107 past the caches too; fp32 no difference).
-#define MT_STREAM_BYTES 256e6
+// What a call streams through, and holds in memory, above this goes past the caches: fp32 parameters, moments and remainders of a
+// step, the gradients a clip rewrites.  The last level holds 256 MB, and a training step touches more than its optimizer does.
+// Three models in turn, cached / past the caches, us: step of 4.1 M parameters (65 MB) 22 / 26, 9 M (144 MB) 61 / 53, 20 M 121 / 102,
+// 60 M 361 / 297; with 8-bit moments 9 M (90 MB) 51 / 49, 60 M 292 / 269; clip of 20 M gradients (80 MB) 42 / 46, 28 M 62 / 60, 60 M
+// 137 / 116.  What stays cached in any case: gradients that the norm has just read and the step reads again, the norm's
+// own reads (past the caches: step of 69.8 M 385 against 343), and bf16 parameters, whose accesses are half as wide (151 against 147).
+#define MT_STREAM_BYTES 96e6
 
 struct MtJob {
     void* p;
@@ -129,10 +130,10 @@ __device__ __forceinline__ void st(T* p, T x) {
 }
 
 // four consecutive elements at p + o, of which the tensor has `left` (FULL: four); what it has not reads as 0 and is not written
-template <bool FULL>
+template <bool FULL, bool NT>
 __device__ __forceinline__ void load4(const float* p, uint32_t o, int left, float x[4]) {
     if (FULL || left >= 4) {
-        const f32x4u q = *(const f32x4u*)(p + o);
+        const f32x4u q = NT ? __builtin_nontemporal_load((const f32x4u*)(p + o)) : *(const f32x4u*)(p + o);
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = q[k];
     } else {
@@ -140,46 +141,48 @@ __device__ __forceinline__ void load4(const float* p, uint32_t o, int left, floa
         for (int k = 0; k < 4; ++k) x[k] = k < left ? p[o + k] : 0.f;
     }
 }
-template <bool FULL>
+template <bool FULL, bool NT>
 __device__ __forceinline__ void load4(const bf16_t* p, uint32_t o, int left, u16x4u& x) {
     if (FULL || left >= 4) {
-        x = *(const u16x4u*)(p + o);
+        x = NT ? __builtin_nontemporal_load((const u16x4u*)(p + o)) : *(const u16x4u*)(p + o);
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = k < left ? p[o + k] : (bf16_t)0;
     }
 }
-template <bool BF, bool FULL>
+template <bool BF, bool FULL, bool NT>
 __device__ __forceinline__ void load4(const void* p, uint32_t o, int left, float x[4]) {
     if (BF) {
         u16x4u q;
-        load4<FULL>((const bf16_t*)p, o, left, q);
+        load4<FULL, NT>((const bf16_t*)p, o, left, q);
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = bf2f(q[k]);
     } else {
-        load4<FULL>((const float*)p, o, left, x);
+        load4<FULL, NT>((const float*)p, o, left, x);
     }
 }
-template <bool FULL>
+template <bool FULL, bool NT>
 __device__ __forceinline__ void store4(float* p, uint32_t o, int left, const float x[4]) {
     if (FULL || left >= 4) {
         f32x4u q;
 #pragma unroll
         for (int k = 0; k < 4; ++k) q[k] = x[k];
-        *(f32x4u*)(p + o) = q;
+        if (NT) __builtin_nontemporal_store(q, (f32x4u*)(p + o));
+        else *(f32x4u*)(p + o) = q;
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
             if (k < left) p[o + k] = x[k];
     }
 }
-template <bool FULL>
+template <bool FULL, bool NT>
 __device__ __forceinline__ void store4(bf16_t* p, uint32_t o, int left, const bf16_t x[4]) {
     if (FULL || left >= 4) {
         u16x4u q;
 #pragma unroll
         for (int k = 0; k < 4; ++k) q[k] = x[k];
-        *(u16x4u*)(p + o) = q;
+        if (NT) __builtin_nontemporal_store(q, (u16x4u*)(p + o));
+        else *(u16x4u*)(p + o) = q;
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -199,10 +202,10 @@ __device__ __forceinline__ void sumsq_chunk(const void* g, long c0, long n, doub
     float x[SQ_DEEP][4];
     if (left == SQ_CHUNK) {
 #pragma unroll
-        for (int u = 0; u < SQ_DEEP; ++u) load4<BF, true>(p, (u * SQ_THREADS + threadIdx.x) * 4u, 0, x[u]);
+        for (int u = 0; u < SQ_DEEP; ++u) load4<BF, true, false>(p, (u * SQ_THREADS + threadIdx.x) * 4u, 0, x[u]);
     } else {
 #pragma unroll
-        for (int u = 0; u < SQ_DEEP; ++u) load4<BF, false>(p, (u * SQ_THREADS + threadIdx.x) * 4u, left - (int)((u * SQ_THREADS + threadIdx.x) * 4u), x[u]);
+        for (int u = 0; u < SQ_DEEP; ++u) load4<BF, false, false>(p, (u * SQ_THREADS + threadIdx.x) * 4u, left - (int)((u * SQ_THREADS + threadIdx.x) * 4u), x[u]);
     }
 #pragma unroll
     for (int u = 0; u < SQ_DEEP; ++u)
@@ -285,11 +288,11 @@ __device__ __forceinline__ float clip_coef(const MtClip& c) {
     return (float)(q >= 1.0 ? 1.0 : q) * c.grad_mul;
 }
 
-template <bool BF, bool FULL>
+template <bool BF, bool FULL, bool NT>
 __device__ __forceinline__ void scale_run(void* g, int left, float coef) {
     float x[4][4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) load4<BF, FULL>(g, (u * 256 + threadIdx.x) * 4u, left - (int)((u * 256 + threadIdx.x) * 4u), x[u]);
+    for (int u = 0; u < 4; ++u) load4<BF, FULL, NT>(g, (u * 256 + threadIdx.x) * 4u, left - (int)((u * 256 + threadIdx.x) * 4u), x[u]);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
         const uint32_t o = (u * 256 + threadIdx.x) * 4u;
@@ -297,21 +300,22 @@ __device__ __forceinline__ void scale_run(void* g, int left, float coef) {
             bf16_t y[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) y[k] = f2bf(x[u][k] * coef);
-            store4<FULL>((bf16_t*)g, o, left - (int)o, y);
+            store4<FULL, NT>((bf16_t*)g, o, left - (int)o, y);
         } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k) x[u][k] *= coef;
-            store4<FULL>((float*)g, o, left - (int)o, x[u]);
+            store4<FULL, NT>((float*)g, o, left - (int)o, x[u]);
         }
     }
 }
-template <bool BF>
+template <bool BF, bool NT>
 __device__ __forceinline__ void scale_chunk(void* g, long c0, long n, float coef) {
     void* p = (char*)g + c0 * (BF ? 2 : 4);
-    if (n - c0 >= MT_CHUNK) scale_run<BF, true>(p, MT_CHUNK, coef);
-    else scale_run<BF, false>(p, (int)(n - c0), coef);
+    if (n - c0 >= MT_CHUNK) scale_run<BF, true, NT>(p, MT_CHUNK, coef);
+    else scale_run<BF, false, NT>(p, (int)(n - c0), coef);
 }
 
+template <bool NT>
 __global__ __launch_bounds__(256) void multi_scale_kernel(const MtTable tab, const MtClip clip) {
     const MtFind find(tab);
     const float coef = clip_coef(clip);
@@ -320,8 +324,8 @@ __global__ __launch_bounds__(256) void multi_scale_kernel(const MtTable tab, con
         const int j = find(c);
         const MtJob& jb = tab.job[j];
         const long c0 = (long)(c - tab.first[j]) * MT_CHUNK;
-        if (jb.slot_flags & VAE_MT_GRAD_BF16) scale_chunk<true>((void*)jb.g, c0, jb.n, coef);
-        else scale_chunk<false>((void*)jb.g, c0, jb.n, coef);
+        if (jb.slot_flags & VAE_MT_GRAD_BF16) scale_chunk<true, NT>((void*)jb.g, c0, jb.n, coef);
+        else scale_chunk<false, NT>((void*)jb.g, c0, jb.n, coef);
     }
 }
 
@@ -398,12 +402,12 @@ struct AdamBlock {
     // whole chunk)
     template <bool FULL>
     __device__ __forceinline__ void load(const MtChunk& c, uint32_t o, int left) {
-        load4<GB, FULL>(c.g, o, left, g);
+        load4<GB, FULL, false>(c.g, o, left, g);
         if (PB) {
-            load4<FULL>((const bf16_t*)c.p, o, left, pb);
+            load4<FULL, false>((const bf16_t*)c.p, o, left, pb);
             r = ld<NT>((const short4v*)(c.rem + o));
         } else {
-            load4<false, FULL>(c.p, o, left, p);
+            load4<false, FULL, NT>(c.p, o, left, p);
         }
         if (S8) {
             qm = ld<NT>((const uint32_t*)((const uint8_t*)c.m + o));
@@ -457,23 +461,26 @@ struct AdamBlock {
             }
         }
         const uint32_t bm = (uint32_t)max(level_up(wave_max_u32(xm)) - 127, 0), bv = (uint32_t)max(level_up(wave_max_u32(xv)) - 254, 0);
-        const float low = __uint_as_float((bm + 1) << 20), unit = low * 0x1p-20f;
-        uint32_t u = i * DITHER_I;
-        qm = odd_m;
-        qv = odd_v;
+        const uint32_t low = (bm + 1) << 20, minus_m = 0u - (bm << 20), minus_v = 0u - (bv << 20);
+        const float unit = __uint_as_float(low) * 0x1p-20f;
+        uint32_t u = i * DITHER_I, cm[4], cv[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k, u += DITHER_I) {
             const uint32_t x = __float_as_uint(m[k]) & 0x7FFFFFFFu, y = __float_as_uint(v[k]);
             const uint32_t dm = NEAR ? 1u << 19 : (u + phase_m) >> 12, dv = NEAR ? 1u << 19 : (u + phase_v) >> 12;
-            const float a = __uint_as_float(x);
             // below the smallest level that has a code: 0 or that level, the latter with probability |m| / low over the
-            // dither (d * unit is exact: 20 bits times 4)
-            uint32_t c = a > (float)dm * unit ? 1u : 0u;
-            c = a >= low ? ((x + dm) >> 20) - bm : c;
-            qm |= (c ? c | ((__float_as_uint(m[k]) >> 24) & 128u) : 0u) << 8 * k;
-            const uint32_t e = (uint32_t)max((int)((y + dv) >> 20) - (int)bv, 1);
-            qv |= (y ? e : 0u) << 8 * k;
+            // dither (d * unit is exact: 20 bits times 4).  Both sides are worked out: a branch would cost more.
+            uint32_t small = __uint_as_float(x) > (float)dm * unit ? 1u : 0u, big = (x + dm + minus_m) >> 20;
+            asm("" : "+v"(small), "+v"(big));
+            cm[k] = x >= low ? big : small;
+            cv[k] = (uint32_t)max((int)(y + dv + minus_v) >> 20, (int)min(y, 1u));      // at least 1 unless y is 0
         }
+        // the four codes in a word, and the signs of those that are not 0: adding 127 carries into bit 7 of every byte from 1 to 127
+        const uint32_t c = cm[0] | cm[1] << 8 | cm[2] << 16 | cm[3] << 24;
+        const uint32_t sign = __builtin_amdgcn_perm(__builtin_amdgcn_perm(__float_as_uint(m[3]), __float_as_uint(m[2]), 0x07030C0Cu),
+                                                    __builtin_amdgcn_perm(__float_as_uint(m[1]), __float_as_uint(m[0]), 0x0C0C0703u), 0x07060100u);
+        qm = c | ((c + 0x7F7F7F7Fu) & sign & 0x80808080u) | odd_m;
+        qv = cv[0] | cv[1] << 8 | cv[2] << 16 | cv[3] << 24 | odd_v;
         return bm | bv << 16;
     }
 
@@ -509,10 +516,10 @@ struct AdamBlock {
                 split_master(p[k], q[k], rk);
                 r[k] = rk;
             }
-            store4<FULL>((bf16_t*)c.p, o, left, q);
+            store4<FULL, false>((bf16_t*)c.p, o, left, q);
             st<NT>((short4v*)(c.rem + o), r);
         } else {
-            store4<FULL>((float*)c.p, o, left, p);
+            store4<FULL, NT>((float*)c.p, o, left, p);
         }
         if (S8) {
             const uint32_t bases = pack<false>(s.phase_m, s.phase_v, i);
@@ -587,10 +594,10 @@ __device__ __forceinline__ void master_chunk(const MtChunk& c, float* out, int l
         const uint32_t o = (u * 256 + threadIdx.x) * 4u;
         if (!FULL && (int)(o & ~(MT_BLOCK - 1u)) >= left) break;       // a block behind the tensor's last is another tensor's
         if (PB) {
-            load4<FULL>((const bf16_t*)c.p, o, left - (int)o, p[u]);
+            load4<FULL, false>((const bf16_t*)c.p, o, left - (int)o, p[u]);
             r[u] = *(const short4v*)(c.rem + o);
         } else {
-            load4<FULL>((const float*)c.p, o, left - (int)o, w[u]);
+            load4<FULL, false>((const float*)c.p, o, left - (int)o, w[u]);
         }
     }
 #pragma unroll
@@ -709,6 +716,11 @@ static double elem_bytes(const MtTable& t, int per_grad_f32) {
     for (int k = 0; k < t.count; ++k) b += (double)t.job[k].n * ((t.job[k].slot_flags & VAE_MT_GRAD_BF16) ? per_grad_f32 / 2 : per_grad_f32);
     return b;
 }
+static double grad_bytes(const vae_mt_tensor* t, int count) {
+    double b = 0;
+    for (int k = 0; k < count; ++k) b += (double)t[k].n * ((t[k].flags & VAE_MT_GRAD_BF16) ? 2 : 4);
+    return b;
+}
 static double elem_count(const MtTable& t) {
     double n = 0;
     for (int k = 0; k < t.count; ++k) n += (double)t.job[k].n;
@@ -778,6 +790,7 @@ extern "C" int vae_multi_clip(const vae_mt_tensor* tensors, int count, double* p
     VAE_CHECK(max_norm >= 0.f, "vae_multi_clip: max_norm=%g must not be negative or NaN", (double)max_norm);
     if (chunks == 0) return vae_multi_grad_norm(tensors, count, partial, grad_mul, norm_out, stream);
     hipStream_t s = (hipStream_t)stream;
+    const bool nt = grad_bytes(tensors, count) > MT_STREAM_BYTES;
     int np = 0;
     if (int rc = sumsq_list(tensors, count, chunks, nullptr, true, partial, &np, s)) return rc;
     MtTable tab;
@@ -787,7 +800,8 @@ extern "C" int vae_multi_clip(const vae_mt_tensor* tensors, int count, double* p
         const MtClip clip = {partial, np, grad_mul, max_norm, norm_out};
         {
             ProfScope prof("multi_scale_kernel", 0.0, elem_bytes(tab, 8), s);
-            hipLaunchKernelGGL(multi_scale_kernel, dim3(update_grid(tab.nchunk)), dim3(256), 0, s, tab, clip);
+            if (nt) hipLaunchKernelGGL(multi_scale_kernel<true>, dim3(update_grid(tab.nchunk)), dim3(256), 0, s, tab, clip);
+            else hipLaunchKernelGGL(multi_scale_kernel<false>, dim3(update_grid(tab.nchunk)), dim3(256), 0, s, tab, clip);
         }
         VAE_LAUNCH_CHECK("multi_scale_kernel");
     }
@@ -821,6 +835,14 @@ extern "C" int vae_multi_adamw_step(const vae_mt_group* groups, int ngroups, dou
         all += chunks;
     }
     hipStream_t s = (hipStream_t)stream;
+    // what the step holds in memory, all groups together
+    double bytes = 0.0;
+    for (int k = 0; k < ngroups; ++k)
+        for (int i = 0; i < groups[k].count; ++i) {
+            const vae_mt_tensor& t = groups[k].tensors[i];
+            bytes += (double)t.n * ((t.flags & VAE_MT_GRAD_BF16 ? 2 : 4) + 4 + (groups[k].state_bits == 8 ? 2 : 8));
+        }
+    const bool nt = bytes > MT_STREAM_BYTES;
     int np = 0;
     for (int k = 0; k < ngroups; ++k) {
         const vae_mt_group& q = groups[k];
@@ -831,13 +853,6 @@ extern "C" int vae_multi_adamw_step(const vae_mt_group* groups, int ngroups, dou
         hipLaunchKernelGGL(multi_norm_kernel, dim3(1), dim3(64), 0, s, MtClip{partial, -1, grad_mul, -1.f, norm_out});
         VAE_LAUNCH_CHECK("multi_norm_kernel");
     }
-    // what the step holds in memory, all groups together
-    double bytes = 0.0;
-    for (int k = 0; k < ngroups; ++k)
-        for (int i = 0; i < groups[k].count; ++i) {
-            const vae_mt_tensor& t = groups[k].tensors[i];
-            bytes += (double)t.n * ((t.flags & VAE_MT_GRAD_BF16 ? 2 : 4) + 4 + (groups[k].state_bits == 8 ? 2 : 8));
-        }
     MtTable tab;
     for (int k = 0; k < ngroups; ++k) {
         const vae_mt_group& q = groups[k];
@@ -848,7 +863,7 @@ extern "C" int vae_multi_adamw_step(const vae_mt_group* groups, int ngroups, dou
             if (!tab.nchunk) continue;
             const MtClip clip = {partial, np, grad_mul, max_norm, norm_out};
             const int grid = update_grid(tab.nchunk);
-            const bool eight = q.state_bits == 8, nt = bytes > MT_STREAM_BYTES;
+            const bool eight = q.state_bits == 8;
             ProfScope prof(eight ? "multi_adamw8_kernel" : "multi_adamw_kernel", 0.0, step_bytes(tab, eight), s);
             if (eight && nt) hipLaunchKernelGGL((multi_adamw_kernel<true, true>), dim3(grid), dim3(256), 0, s, tab, h, clip);
             else if (eight) hipLaunchKernelGGL((multi_adamw_kernel<true, false>), dim3(grid), dim3(256), 0, s, tab, h, clip);

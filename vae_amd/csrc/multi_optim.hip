@@ -629,26 +629,29 @@ __global__ __launch_bounds__(256) void multi_master_kernel(const MtTable tab, co
 }
 
 // 8 elements a thread: 16-byte stores
-template <bool BF>
+template <bool BF, bool NT>
 __global__ __launch_bounds__(256) void moments8_unpack_kernel(const uint8_t* __restrict__ qm, const uint8_t* __restrict__ qv,
                                                               const short2* __restrict__ base, void* __restrict__ m, void* __restrict__ v, long n) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (long)gridDim.x * 2048) {
-        const uint2 a = *(const uint2*)(qm + i), c = *(const uint2*)(qv + i);
+        const u32x2 a = ld<NT>((const u32x2*)(qm + i)), c = ld<NT>((const u32x2*)(qv + i));
         const short2 b = base[i / MT_BLOCK];
         float x[8], y[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            x[k] = unpack_m(((k < 4 ? a.x : a.y) >> 8 * (k & 3)) & 255u, b.x);
-            y[k] = unpack_v(((k < 4 ? c.x : c.y) >> 8 * (k & 3)) & 255u, b.y);
+            x[k] = unpack_m((a[k / 4] >> 8 * (k & 3)) & 255u, b.x);
+            y[k] = unpack_v((c[k / 4] >> 8 * (k & 3)) & 255u, b.y);
         }
         if (BF) {      // 4 significant bits: exact
-            *(uint4*)((bf16_t*)m + i) = make_uint4(pack2bf(x[0], x[1]), pack2bf(x[2], x[3]), pack2bf(x[4], x[5]), pack2bf(x[6], x[7]));
-            *(uint4*)((bf16_t*)v + i) = make_uint4(pack2bf(y[0], y[1]), pack2bf(y[2], y[3]), pack2bf(y[4], y[5]), pack2bf(y[6], y[7]));
+            st<NT>((u32x4*)((bf16_t*)m + i), u32x4{pack2bf(x[0], x[1]), pack2bf(x[2], x[3]), pack2bf(x[4], x[5]), pack2bf(x[6], x[7])});
+            st<NT>((u32x4*)((bf16_t*)v + i), u32x4{pack2bf(y[0], y[1]), pack2bf(y[2], y[3]), pack2bf(y[4], y[5]), pack2bf(y[6], y[7])});
         } else {
-            *(float4*)((float*)m + i) = make_float4(x[0], x[1], x[2], x[3]);
-            *(float4*)((float*)m + i + 4) = make_float4(x[4], x[5], x[6], x[7]);
-            *(float4*)((float*)v + i) = make_float4(y[0], y[1], y[2], y[3]);
-            *(float4*)((float*)v + i + 4) = make_float4(y[4], y[5], y[6], y[7]);
+#pragma unroll
+            for (int h = 0; h < 8; h += 4) {
+                st<NT>((f32x4*)((float*)m + i + h), f32x4{x[h], x[h + 1], x[h + 2], x[h + 3]});
+                st<NT>((f32x4*)((float*)v + i + h), f32x4{y[h], y[h + 1], y[h + 2], y[h + 3]});
+            }
         }
     }
 }
@@ -910,12 +913,11 @@ extern "C" int vae_moments8_unpack(const void* exp_avg_q, const void* exp_avg_sq
               "vae_moments8_unpack: buffers must be 16-byte aligned");
     {
         ProfScope prof("moments8_unpack_kernel", 0.0, 256.0 * nblocks * (bf16_out ? 6 : 10), (hipStream_t)stream);
-        if (bf16_out)
-            hipLaunchKernelGGL(moments8_unpack_kernel<true>, dim3(blocks_grid(nblocks, 8)), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)exp_avg_q,
-                               (const uint8_t*)exp_avg_sq_q, (const short2*)bases, exp_avg, exp_avg_sq, nblocks * MT_BLOCK);
-        else
-            hipLaunchKernelGGL(moments8_unpack_kernel<false>, dim3(blocks_grid(nblocks, 8)), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)exp_avg_q,
-                               (const uint8_t*)exp_avg_sq_q, (const short2*)bases, exp_avg, exp_avg_sq, nblocks * MT_BLOCK);
+        const bool nt = 256.0 * nblocks * (bf16_out ? 6 : 10) > MT_STREAM_BYTES;
+        const auto kernel = bf16_out ? (nt ? moments8_unpack_kernel<true, true> : moments8_unpack_kernel<true, false>)
+                                     : (nt ? moments8_unpack_kernel<false, true> : moments8_unpack_kernel<false, false>);
+        hipLaunchKernelGGL(kernel, dim3(blocks_grid(nblocks, 8)), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)exp_avg_q,
+                           (const uint8_t*)exp_avg_sq_q, (const short2*)bases, exp_avg, exp_avg_sq, nblocks * MT_BLOCK);
     }
     VAE_LAUNCH_CHECK("moments8_unpack_kernel");
     return 0;

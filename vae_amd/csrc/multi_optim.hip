@@ -584,7 +584,7 @@ __global__ __launch_bounds__(256) void multi_adamw_kernel(const MtTable tab, con
 }
 
 // masters of the bf16 parameters (and the fp32 parameters themselves) in the state's layout, padding 0
-template <bool PB, bool FULL>
+template <bool PB, bool FULL, bool NT>
 __device__ __forceinline__ void master_chunk(const MtChunk& c, float* out, int left) {
     float w[MT_CHUNK / 1024][4];
     short4v r[MT_CHUNK / 1024];
@@ -595,7 +595,7 @@ __device__ __forceinline__ void master_chunk(const MtChunk& c, float* out, int l
         if (!FULL && (int)(o & ~(MT_BLOCK - 1u)) >= left) break;       // a block behind the tensor's last is another tensor's
         if (PB) {
             load4<FULL, false>((const bf16_t*)c.p, o, left - (int)o, p[u]);
-            r[u] = *(const short4v*)(c.rem + o);
+            r[u] = ld<NT>((const short4v*)(c.rem + o));
         } else {
             load4<FULL, false>((const float*)c.p, o, left - (int)o, w[u]);
         }
@@ -608,9 +608,10 @@ __device__ __forceinline__ void master_chunk(const MtChunk& c, float* out, int l
 #pragma unroll
             for (int k = 0; k < 4; ++k) w[u][k] = FULL || (int)o + k < left ? join_master(p[u][k], r[u][k]) : 0.f;
         }
-        *(f32x4*)(out + o) = f32x4{w[u][0], w[u][1], w[u][2], w[u][3]};
+        st<NT>((f32x4*)(out + o), f32x4{w[u][0], w[u][1], w[u][2], w[u][3]});
     }
 }
+template <bool NT>
 __global__ __launch_bounds__(256) void multi_master_kernel(const MtTable tab, const short* __restrict__ rem, float* __restrict__ out) {
     const MtFind find(tab);
     for (uint32_t c = blockIdx.x; c < tab.nchunk; c += gridDim.x) {
@@ -621,10 +622,10 @@ __global__ __launch_bounds__(256) void multi_master_kernel(const MtTable tab, co
         const bool bf = jb.slot_flags & VAE_MT_PARAM_BF16, full = jb.n - c0 >= MT_CHUNK;
         const int left = full ? MT_CHUNK : (int)(jb.n - c0);
         MtChunk k = {(char*)jb.p + c0 * (bf ? 2 : 4), nullptr, nullptr, nullptr, (short*)rem + k0, nullptr};
-        if (bf && full) master_chunk<true, true>(k, out + k0, left);
-        else if (bf) master_chunk<true, false>(k, out + k0, left);
-        else if (full) master_chunk<false, true>(k, out + k0, left);
-        else master_chunk<false, false>(k, out + k0, left);
+        if (bf && full) master_chunk<true, true, NT>(k, out + k0, left);
+        else if (bf) master_chunk<true, false, NT>(k, out + k0, left);
+        else if (full) master_chunk<false, true, NT>(k, out + k0, left);
+        else master_chunk<false, false, NT>(k, out + k0, left);
     }
 }
 
@@ -891,7 +892,8 @@ extern "C" int vae_multi_master(const vae_mt_tensor* tensors, int count, const s
         if (!tab.nchunk) continue;
         {
             ProfScope prof("multi_master_kernel", 0.0, 8.0 * elem_count(tab), (hipStream_t)stream);
-            hipLaunchKernelGGL(multi_master_kernel, dim3(update_grid(tab.nchunk)), dim3(256), 0, (hipStream_t)stream, tab, remainder, out);
+            const auto kernel = 2048.0 * nblocks > MT_STREAM_BYTES ? multi_master_kernel<true> : multi_master_kernel<false>;
+            hipLaunchKernelGGL(kernel, dim3(update_grid(tab.nchunk)), dim3(256), 0, (hipStream_t)stream, tab, remainder, out);
         }
         VAE_LAUNCH_CHECK("multi_master_kernel");
     }

@@ -316,3 +316,18 @@ def test_the_extension_is_refused_under_another_torch(monkeypatch):
     monkeypatch.setattr(L, "HOST_PATH", "/nowhere/_host.so")
     with pytest.raises(RuntimeError, match="not found"):
         L.host()
+
+
+def test_each_thread_has_a_table_of_its_own():
+    import threading
+    t, seen = optim._tables, []
+    t.room(100)
+    mine = t.addr
+    assert len(t.jobs) >= 100 and t.jobs.ctypes.data == mine and t.room(3) is t.jobs
+
+    def other():
+        seen.append((t.room(10).ctypes.data, t.addr))
+    th = threading.Thread(target=other)
+    th.start()
+    th.join()
+    assert seen[0][0] == seen[0][1] != mine and t.addr == mine

@@ -7,6 +7,7 @@ eps 1e-8, weight_decay 0.01) preceded by clip_grad_norm_(max_norm) (train.py:336
 from __future__ import annotations
 
 import ctypes
+import threading
 
 import numpy as np
 import torch
@@ -79,17 +80,39 @@ def _dense(t):
     return True
 
 
+class _Tables(threading.local):
+    """Each thread's table for the calls that keep none: the library has read it when a call returns."""
+    jobs, addr = np.empty(0, _JOB), 0
+
+    def room(self, n):
+        if len(self.jobs) < n:
+            self.jobs = np.empty(max(64, 2 * n), _JOB)
+            self.addr = self.jobs.ctypes.data
+        return self.jobs
+
+
+_tables = _Tables()
+
+
 def _grad_jobs(parameters, who, write):
-    """(table of the parameters' gradients, their number, one of them or None).  ``write``: they are written in place"""
+    """(address of the table of the parameters' gradients, their number, what has to live until the launch).  ``write``: they are
+    written in place"""
     params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    first = next((p.grad for p in params if p.grad is not None), None)
+    first = None
+    for p in params:
+        first = p.grad
+        if first is not None:
+            break
     if first is None:
-        return None, 0, None
+        return 0, 0, None
     _lib.check_device(first)
-    jobs = np.empty(len(params), _JOB)
+    jobs = _tables.room(len(params))
     n = _lib.host().collect_grads(params, jobs, first.get_device(), write)
-    if n >= 0:
-        return jobs, n, first
+    return (_tables.addr, n, first) if n >= 0 else _grad_jobs_general(params, first, who, write)
+
+
+@torch.no_grad()
+def _grad_jobs_general(params, first, who, write):
     grads = [p.grad for p in params if p.grad is not None]
     for g in grads:
         if g.layout is not torch.strided or g.dtype not in _TYPES:
@@ -107,27 +130,25 @@ def _grad_jobs(parameters, who, write):
         increment_version(grads)
     else:
         grads = [g if _dense(g) else g.contiguous() for g in grads]
-    jobs["grad"][:len(grads)] = [g.data_ptr() for g in grads]
-    jobs["n"][:len(grads)] = [g.numel() for g in grads]
-    jobs["flags"][:len(grads)] = [_lib.MT_GRAD_BF16 if g.dtype is torch.bfloat16 else 0 for g in grads]
-    return jobs, len(grads), grads
+    jobs = np.zeros(len(grads), _JOB)
+    jobs["grad"] = [g.data_ptr() for g in grads]
+    jobs["n"] = [g.numel() for g in grads]
+    jobs["flags"] = [_lib.MT_GRAD_BF16 if g.dtype is torch.bfloat16 else 0 for g in grads]
+    return jobs.ctypes.data, len(grads), (jobs, grads)
 
 
-@torch.no_grad()
 def grad_norm(parameters):
     """Global L2 norm of the parameters' gradients as a 0-dim fp32 tensor: one launch per 192 tensors and one that finishes the
     sum.  Squares and sums in 64 bits, in a fixed order."""
     jobs, n, keep = _grad_jobs(parameters, "grad_norm", False)
     if n == 0:
         return torch.zeros(())
-    dev = torch.device("cuda", torch.cuda.current_device())
-    partial = torch.empty(_lib.call("vae_multi_partials", n), dtype=torch.float64, device=dev)
-    out = torch.empty((), device=dev)
-    _lib.call("vae_multi_grad_norm", jobs.ctypes.data, n, partial.data_ptr(), 1.0, out.data_ptr(), _lib.current_stream())
+    partial = torch.empty(_lib.call("vae_multi_partials", n), dtype=torch.float64, device="cuda")
+    out = torch.empty((), device="cuda")
+    _lib.call("vae_multi_grad_norm", jobs, n, partial.data_ptr(), 1.0, out.data_ptr(), _lib.current_stream())
     return out
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """torch.nn.utils.clip_grad_norm_ (vae/training/train.py:336) for fp32 and bf16 gradients of any number of tensors: scales
     them in place by ``min(1, max_norm / (norm + 1e-6))`` and returns the norm before that as a 0-dim fp32 tensor.  Two launches per
@@ -135,7 +156,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grad_norm_: max_norm={max_norm} must not be negative or NaN")
-    if float(norm_type) != 2.0:
+    if norm_type != 2.0 and float(norm_type) != 2.0:
         raise ValueError(f"clip_grad_norm_: norm_type={norm_type}; only the L2 norm is computed")
     if error_if_nonfinite:
         parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
@@ -145,10 +166,9 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     jobs, n, keep = _grad_jobs(parameters, "clip_grad_norm_", True)
     if n == 0:
         return torch.zeros(())
-    dev = torch.device("cuda", torch.cuda.current_device())
-    partial = torch.empty(_lib.call("vae_multi_partials", n), dtype=torch.float64, device=dev)
-    out = torch.empty((), device=dev)
-    _lib.call("vae_multi_clip", jobs.ctypes.data, n, partial.data_ptr(), 1.0, max_norm, out.data_ptr(), _lib.current_stream())
+    partial = torch.empty(_lib.call("vae_multi_partials", n), dtype=torch.float64, device="cuda")
+    out = torch.empty((), device="cuda")
+    _lib.call("vae_multi_clip", jobs, n, partial.data_ptr(), 1.0, max_norm, out.data_ptr(), _lib.current_stream())
     return out
 
 
@@ -180,6 +200,7 @@ class _GroupState:
         self.steps = z(len(params), dtype=torch.int64)
         self.scalars = z(len(params), 8)
         self.jobs = np.zeros(len(params), _JOB)
+        self.jobs_addr = self.jobs.ctypes.data
         self.index = self.device.index
         self.param_flags = [_lib.MT_PARAM_BF16 if d is torch.bfloat16 else 0 for d in self.dtypes]
         self.layout = np.stack([self.n, self.start, np.arange(len(params)), self.param_flags], 1).astype(np.int64)
@@ -203,7 +224,7 @@ class _GroupState:
         """fills the table of the tensors that have a gradient; returns their number and what has to live until the launch"""
         n = _lib.host().collect_step(self.params, self.jobs, self.layout, self.index)
         if n >= 0:
-            self.c.tensors, self.c.count = self.jobs.ctypes.data, n
+            self.c.tensors, self.c.count = self.jobs_addr, n
             return n, None
         ptrs, gptrs, flags, keep, live, at = [], [], [], [], [], []
         for k, p in enumerate(self.params):
@@ -405,22 +426,24 @@ class MultiAdamW(torch.optim.Optimizer):
         _lib.call("vae_moments8_unpack", qm.data_ptr(), qv.data_ptr(), bases.data_ptr(), m.data_ptr(), v.data_ptr(), bases.shape[0],
                   int(m.dtype is torch.bfloat16), _lib.current_stream())
 
-    @torch.no_grad()
     def flat_master(self, group=0):
         """32-bit values of a group's parameters in the state's layout: a bf16 parameter's master, an fp32 parameter itself"""
         st = self._groups[group]
         _lib.check_device(st.exp_avg)
         # every block is some tensor's and is written whole
         out = (torch.empty if st.nblocks else torch.zeros)(max(st.nblocks, 1) * _lib.MT_BLOCK, device=st.device)
-        jobs = np.zeros(len(st.params), _JOB)
+        jobs = _tables.room(len(st.params))
+        addr = _tables.addr
         if _lib.host().collect_params(st.params, jobs, st.layout, st.index) < 0:
+            jobs = np.zeros(len(st.params), _JOB)
+            addr = jobs.ctypes.data
             for k in range(len(st.params)):
                 st.check_param(k)
             jobs["n"], jobs["block"], jobs["slot"] = st.layout[:, 0], st.layout[:, 1], st.layout[:, 2]
             jobs["param"] = [p.data_ptr() for p in st.params]
             jobs["grad"] = jobs["param"]       # not read
             jobs["flags"] = [f * (_lib.MT_PARAM_BF16 | _lib.MT_GRAD_BF16) for f in st.param_flags]
-        _lib.call("vae_multi_master", jobs.ctypes.data, len(st.params), _lib.ptr(st.remainder), out.data_ptr(), st.nblocks, _lib.current_stream())
+        _lib.call("vae_multi_master", addr, len(st.params), _lib.ptr(st.remainder), out.data_ptr(), st.nblocks, _lib.current_stream())
         return out
 
     @torch.no_grad()

@@ -620,7 +620,8 @@ int vae_multi_clip(const vae_mt_tensor* tensors, int count, double* partial, flo
  * written).  The norm runs over all groups.  max_norm < 0: no clipping, and with norm_out = NULL no norm is taken. */
 int vae_multi_adamw_step(const vae_mt_group* groups, int ngroups, double* partial, float grad_mul, float max_norm, float* norm_out,
                          void* stream);
-/* out[block * 256 + k] = 32-bit value of parameter element k (master of a bf16 parameter); padding of listed tensors = 0 */
+/* out[block * 256 + k] = 32-bit value of parameter element k (master of a bf16 parameter); padding of listed tensors = 0.
+ * Gradients are not looked at. */
 int vae_multi_master(const vae_mt_tensor* tensors, int count, const short* remainder, float* out, long nblocks, void* stream);
 /* 8-bit moments -> fp32, or (bf16_out) bf16, which holds their values exactly */
 int vae_moments8_unpack(const void* exp_avg_q, const void* exp_avg_sq_q, const short* bases, void* exp_avg, void* exp_avg_sq,

@@ -335,6 +335,86 @@ def test_extreme_values(O):
         assert bool((p.abs() <= 5 * 1e-3 * (1 + 1e-5)).all())       # |m| <= sqrt(v): five steps of at most lr with a constant gradient
 
 
+def test_a_norm_that_is_nan_leaves_the_padding_alone(O):
+    for bits in (32, 8):
+        p = torch.nn.Parameter(torch.ones(300, device=DEV))
+        opt = O.MultiAdamW([p], state_bits=bits)
+        p.grad = torch.ones(300, device=DEV)
+        p.grad[7] = float("nan")
+        opt.step(max_norm=1.0)
+        assert bool(torch.isnan(p).all()) and bool(torch.isnan(opt.grad_norm))       # as clip_grad_norm_ and step() of torch
+        for flat in (*opt.flat_moments(), opt.flat_master()):
+            assert not bool(flat[300:].any())
+
+
+@pytest.mark.parametrize("pd, bits", [(F32, 8), (BF16, 32)])
+def test_offsets_beyond_32_bits(O, pd, bits):
+    """one tensor of more than 2^31 elements: its last ones are stepped like the same ones of a small tensor, its first ones too"""
+    n, m = (1 << 31) + 4097, 5000
+    p = torch.nn.Parameter(torch.full((n,), 0.5, dtype=pd, device=DEV))
+    p.grad = torch.zeros(n, dtype=pd, device=DEV)
+    g = torch.randn(m, device=DEV).to(pd)
+    p.grad[:m], p.grad[-m:] = g, g
+    q = torch.nn.Parameter(torch.full((m,), 0.5, dtype=pd, device=DEV))
+    q.grad = g.clone()
+    a, b = O.MultiAdamW([p], lr=1e-2, state_bits=bits), O.MultiAdamW([q], lr=1e-2, state_bits=bits)
+    norm = R.norm([np64(g)]) * np.sqrt(2.0)
+    a.step(max_norm=1.0)
+    b.grad_mul = R.coefficient(norm, 1.0)
+    b.step()
+    assert abs(float(a.grad_norm) - norm) <= 1.01 * R.EPS24 * norm
+    # coef is the same number rounded to fp32 in both, so the small tensor's bits are the large one's
+    assert torch.equal(p[:m], q) and torch.equal(p[-m:], q)
+    mid = p[m:m + 100].float()
+    assert bool((mid == mid[0]).all())       # no gradient there: the decay alone
+    del a, p
+    torch.cuda.empty_cache()
+
+
+def test_a_group_added_after_a_capture_leaves_the_graph_alone(O):
+    p, q = (torch.nn.Parameter(torch.ones(5000, device=DEV)) for _ in range(2))
+    a, b = O.MultiAdamW([p], lr=1e-2), O.MultiAdamW([q], lr=1e-2)
+    p.grad, q.grad = torch.randn(5000, device=DEV), None
+    q.grad = p.grad.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step(max_norm=1.0)
+    a.add_param_group({"params": [torch.nn.Parameter(torch.ones(40_000, device=DEV))]})
+    fill = [torch.full((321,), 3.0, dtype=torch.float64, device=DEV) for _ in range(64)]       # what a freed scratch would be given to
+    for _ in range(3):
+        graph.replay()
+        b.step(max_norm=1.0)
+        torch.cuda.synchronize()
+        assert torch.equal(p, q)
+    assert all(bool((x == 3).all()) for x in fill)
+
+
+def test_state_dicts_that_do_not_fit_change_nothing(O):
+    p = torch.nn.Parameter(torch.randn(700, device=DEV))
+    opt = O.MultiAdamW([p], state_bits=8)
+    p.grad = torch.randn(700, device=DEV)
+    opt.step()
+    kept, lr = [x.clone() for x in opt.flat_moments()], opt.param_groups[0]["lr"]
+
+    def broken(key, value):
+        sd = copy.deepcopy(opt.state_dict())
+        sd["param_groups"][0]["lr"] = 7.0
+        sd["state"][0][key] = value
+        return sd
+    for key, value, match in (("step", -1.0, "step count"), ("step", 1.5, "step count"), ("step", float("nan"), "step count"),
+                              ("exp_avg_base", torch.full((3,), 3000, dtype=torch.int32), "no levels"),
+                              ("exp_avg_sq_base", torch.full((3,), -5, dtype=torch.int32), "no levels"),
+                              ("exp_avg_q", torch.zeros(699, dtype=torch.uint8), "exp_avg_q"), ("stride", (2,), "order of strides")):
+        with pytest.raises((ValueError, RuntimeError), match=match):
+            sd = broken(key, value)
+            if "base" in key:       # both on one device
+                for k2 in ("exp_avg_base", "exp_avg_sq_base"):
+                    sd["state"][0][k2] = sd["state"][0][k2].cpu()
+            opt.load_state_dict(sd)
+        assert all(torch.equal(x, y) for x, y in zip(opt.flat_moments(), kept)) and opt.param_groups[0]["lr"] == lr
+        assert float(state_of(opt)["step"]) == 1
+
+
 def test_memory_orders_and_expanded_gradients(O):
     a = torch.nn.Parameter(torch.randn(8, 6, 3, 3, device=DEV).to(memory_format=torch.channels_last))
     b = torch.nn.Parameter(a.detach().contiguous().clone())

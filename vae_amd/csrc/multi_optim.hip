@@ -497,6 +497,7 @@ struct AdamBlock {
             const float gk = g[k] * coef;
             m[k] = h.b1 * m[k] + h.omb1 * gk;
             v[k] = h.b2 * v[k] + h.omb2 * gk * gk;
+            if (!FULL && k >= left) m[k] = v[k] = 0.f;       // the padding stays 0 under a coefficient that is NaN too
         }
         if (S8) {
 #pragma unroll
@@ -678,14 +679,14 @@ __global__ __launch_bounds__(256) void moments8_pack_kernel(const float* __restr
 
 // ---------------------------------------------------------------- host
 // *sq_chunks: what the norm's workgroups take in turn, over all tensors
-static int check_tensors(const char* who, const vae_mt_tensor* t, int count, bool params, long nblocks, int nslots, long* sq_chunks) {
+static int check_tensors(const char* who, const vae_mt_tensor* t, int count, bool grads, bool params, long nblocks, int nslots, long* sq_chunks) {
     VAE_CHECK(count >= 0 && count <= VAE_MT_MAX_TENSORS && (t || count == 0), "%s: count=%d out of range (0..%d)", who, count, VAE_MT_MAX_TENSORS);
     long total = 0, sq = 0;
     for (int i = 0; i < count; ++i) {
         VAE_CHECK(t[i].n >= 0 && t[i].n < (1L << 40), "%s: tensor %d has n=%ld", who, i, t[i].n);
         VAE_CHECK((t[i].flags & ~3u) == 0, "%s: tensor %d has unknown flags 0x%x", who, i, t[i].flags);
         if (t[i].n == 0) continue;
-        VAE_CHECK(t[i].grad && ((uintptr_t)t[i].grad & ((t[i].flags & VAE_MT_GRAD_BF16) ? 1 : 3)) == 0,
+        VAE_CHECK(!grads || (t[i].grad && ((uintptr_t)t[i].grad & ((t[i].flags & VAE_MT_GRAD_BF16) ? 1 : 3)) == 0),
                   "%s: tensor %d: gradient is null or not aligned to its type", who, i);
         if (params) {
             VAE_CHECK(t[i].param && ((uintptr_t)t[i].param & ((t[i].flags & VAE_MT_PARAM_BF16) ? 1 : 3)) == 0,
@@ -776,7 +777,7 @@ extern "C" int vae_multi_partials(int count) {
 
 extern "C" int vae_multi_grad_norm(const vae_mt_tensor* tensors, int count, double* partial, float grad_mul, float* norm_out, void* stream) {
     long chunks = 0;
-    if (check_tensors("vae_multi_grad_norm", tensors, count, false, 0, 0, &chunks)) return 1;
+    if (check_tensors("vae_multi_grad_norm", tensors, count, true, false, 0, 0, &chunks)) return 1;
     VAE_CHECK(partial && norm_out, "vae_multi_grad_norm: null pointer");
     hipStream_t s = (hipStream_t)stream;
     int np = 0;
@@ -789,7 +790,7 @@ extern "C" int vae_multi_grad_norm(const vae_mt_tensor* tensors, int count, doub
 
 extern "C" int vae_multi_clip(const vae_mt_tensor* tensors, int count, double* partial, float grad_mul, float max_norm, float* norm_out, void* stream) {
     long chunks = 0;
-    if (check_tensors("vae_multi_clip", tensors, count, false, 0, 0, &chunks)) return 1;
+    if (check_tensors("vae_multi_clip", tensors, count, true, false, 0, 0, &chunks)) return 1;
     VAE_CHECK(partial && norm_out, "vae_multi_clip: null pointer");
     VAE_CHECK(max_norm >= 0.f, "vae_multi_clip: max_norm=%g must not be negative or NaN", (double)max_norm);
     if (chunks == 0) return vae_multi_grad_norm(tensors, count, partial, grad_mul, norm_out, stream);
@@ -829,7 +830,7 @@ extern "C" int vae_multi_adamw_step(const vae_mt_group* groups, int ngroups, dou
         VAE_CHECK(q.eps >= 0.0 && q.weight_decay >= 0.0 && (q.lr_dev || q.lr >= 0.0), "vae_multi_adamw_step: lr=%g, eps=%g and weight_decay=%g must not be negative",
                   q.lr, q.eps, q.weight_decay);
         long chunks = 0;
-        if (check_tensors("vae_multi_adamw_step", q.tensors, q.count, true, q.nblocks, q.nslots, &chunks)) return 1;
+        if (check_tensors("vae_multi_adamw_step", q.tensors, q.count, true, true, q.nblocks, q.nslots, &chunks)) return 1;
         VAE_CHECK(q.count == 0 || (q.steps && q.scalars), "vae_multi_adamw_step: null step counts or scalars");
         VAE_CHECK(chunks == 0 || (q.exp_avg && q.exp_avg_sq && (q.state_bits == 32 || q.bases)), "vae_multi_adamw_step: null state");
         VAE_CHECK((((uintptr_t)q.exp_avg | (uintptr_t)q.exp_avg_sq | (uintptr_t)q.remainder | (uintptr_t)q.bases | (uintptr_t)q.scalars) & 15) == 0,
@@ -885,7 +886,7 @@ extern "C" int vae_multi_master(const vae_mt_tensor* tensors, int count, const s
     VAE_CHECK(count >= 0 && (tensors || count == 0), "vae_multi_master: count=%d", count);
     for (int i = 0; i < count; ++i)
         VAE_CHECK(!(tensors[i].flags & VAE_MT_PARAM_BF16) || tensors[i].n == 0 || remainder, "vae_multi_master: bf16 parameter %d needs the remainder buffer", i);
-    if (check_tensors("vae_multi_master", tensors, count, true, nblocks, 0x7FFFFFFF, &chunks)) return 1;
+    if (check_tensors("vae_multi_master", tensors, count, false, true, nblocks, 0x7FFFFFFF, &chunks)) return 1;
     MtTable tab;
     for (int at = 0; at < count;) {
         at = fill_table(tensors, count, at, MT_CHUNK, tab);

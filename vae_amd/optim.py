@@ -289,7 +289,7 @@ class MultiAdamW(torch.optim.Optimizer):
         self._groups, self._spans = [], []
         self.grad_mul = 1.0
         self.grad_norm = None
-        self._partial = None
+        self._partial, self._old_partials = None, []
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits))
 
     @staticmethod
@@ -344,6 +344,7 @@ class MultiAdamW(torch.optim.Optimizer):
             self.param_groups.pop()
             raise
         n = _lib.call("vae_multi_partials", sum(len(g.params) for g in self._groups))
+        self._old_partials.append(self._partial)       # a graph that captured a step goes on using the one it captured
         self._partial = torch.empty(n, dtype=torch.float64, device=params[0].device)
         if self.grad_norm is None:
             self.grad_norm = torch.zeros(1, device=params[0].device)
@@ -397,6 +398,8 @@ class MultiAdamW(torch.optim.Optimizer):
             (c.beta1, c.beta2), c.eps, c.weight_decay = g["betas"], g["eps"], g["weight_decay"]
             self._c[k] = c
         if total == 0:
+            if clip >= 0.0:
+                self.grad_norm.zero_()
             return
         stream = _lib.current_stream()
         if stream != self._home:
@@ -481,6 +484,11 @@ class MultiAdamW(torch.optim.Optimizer):
             row = [state.get(i, {}) for i in saved["params"]]
             for k, e in enumerate(row):
                 self._check_entry(st, k, e)
+            bases = [e[key].reshape(-1) for e in row if "exp_avg_q" in e for key in ("exp_avg_base", "exp_avg_sq_base")]
+            if bases:
+                low, high = torch.cat(bases).aminmax() if sum(b.numel() for b in bases) else (0, 0)
+                if int(low) < 0 or int(high) > 0x7F7:
+                    raise ValueError(f"MultiAdamW: bases from {int(low)} to {int(high)} are no levels of finite numbers")
             entries.append(row)
         merged = []
         for saved, g in zip(groups, self.param_groups):
@@ -499,7 +507,7 @@ class MultiAdamW(torch.optim.Optimizer):
                     g[key].fill_(x)       # a captured step reads this tensor
                 else:
                     g[key] = x
-            st.steps.copy_(torch.tensor([int(e.get("step", 0)) for e in row], dtype=torch.int64))
+            st.steps.copy_(torch.tensor([int(e.get("step", 0)) for e in row], dtype=torch.int64))       # checked above
             if st.remainder is not None:
                 st.remainder.zero_()
                 have = [k for k, e in enumerate(row) if "remainder" in e and st.dtypes[k] is torch.bfloat16]
@@ -512,6 +520,9 @@ class MultiAdamW(torch.optim.Optimizer):
         def fits(key, numel):
             if key in e and e[key].numel() != numel:
                 raise ValueError(f"MultiAdamW: {key} of parameter {k} has {e[key].numel()} elements where {numel} are wanted")
+        step = float(e.get("step", 0))
+        if not 0.0 <= step < 2.0 ** 62 or step != int(step):
+            raise ValueError(f"MultiAdamW: the step count of parameter {k} is {step}")
         if ("exp_avg" in e) != ("exp_avg_sq" in e) or ("exp_avg" in e and "exp_avg_q" in e):
             raise ValueError(f"MultiAdamW: the entry of parameter {k} has {sorted(e)}")
         for key in ("exp_avg", "exp_avg_sq", "exp_avg_q", "exp_avg_sq_q", "remainder"):

@@ -605,7 +605,7 @@ typedef struct {
     short* remainder;        /* short[nblocks * 256] where a parameter is bf16 */
     long nblocks;
     long* steps;             /* device long[nslots]: steps taken; advanced by the call */
-    float* scalars;          /* device scratch, 8 floats per slot */
+    float* scalars;          /* device scratch, 8 floats per slot, zero before the first call */
     const float* lr_dev;     /* optional device float that is read instead of lr */
     double lr, beta1, beta2, eps, weight_decay;
 } vae_mt_group;

@@ -52,6 +52,11 @@ namespace vae {
 // own reads (past the caches: step of 69.8 M 385 against 343), and bf16 parameters, whose accesses are half as wide (151 against 147).
 #define MT_STREAM_BYTES 96e6
 
+// Up to this many chunks (four workgroups per CU, all of them running at once) a step without a norm is one launch: 39 k parameters in 8
+// tensors 8.7 us as called from Python against 12.4.  Above, waiting for its numbers in every workgroup costs more than the launch
+// that prepares them: 69.8 M parameters with 8-bit moments 212 us against 185.
+#define MT_OWN_CHUNKS 1024
+
 struct MtJob {
     void* p;
     const void* g;
@@ -79,7 +84,7 @@ struct MtPrep {
     const float* lr_dev;
     double lr, b1, b2, wd;
 };
-// per-tensor numbers of a step, 8 floats at scal + 8 * slot
+// per-tensor numbers of a step, at scal + 8 * slot
 struct MtScal {
     float decay, step, inv_bc2;
     uint32_t phase_m, phase_v;
@@ -101,6 +106,9 @@ struct MtChunk {
 // vectors whose address is only as aligned as one element: the memory system takes any 4-byte (fp32) or 2-byte (bf16) address
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned short u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+
+// chunks of a tensor in the step's launch: an empty one has one too, which advances its step count
+__host__ __device__ __forceinline__ uint32_t mt_chunks(long n) { return n ? (uint32_t)((n + MT_CHUNK - 1) / MT_CHUNK) : 1u; }
 
 // Which tensor a chunk belongs to: the last one whose first chunk is not behind it.  All lanes compare at once.
 struct MtFind {
@@ -223,21 +231,40 @@ __device__ __forceinline__ double int_pow(double b, unsigned long t) {
     return r;
 }
 
-// Advances each tensor's step count and works out what depends on it alone, in 64 bits.  The counts live on the device, so
-// that a captured step counts on when it is replayed.
+// What depends on a tensor's step count alone, in 64 bits.  The counts live on the device, so that a captured step counts on when
+// it is replayed.
+__device__ __forceinline__ MtScal step_numbers(const MtPrep& h, long t) {
+    const double lr = h.lr_dev ? (double)*h.lr_dev : h.lr;
+    return {(float)(1.0 - lr * h.wd), (float)(lr / (1.0 - int_pow(h.b1, t))), (float)(1.0 / sqrt(1.0 - int_pow(h.b2, t))), (uint32_t)t * DITHER_M,
+            (uint32_t)t * DITHER_V};
+}
+// beside the norm's workgroups: advances the counts and leaves the numbers for the step's launch
 __device__ __forceinline__ void prep_tensors(const MtTable& tab, const MtPrep& h) {
     for (int i = threadIdx.x; i < tab.count; i += blockDim.x) {
         const uint32_t slot = tab.job[i].slot_flags >> 2;
         const long t = h.steps[slot] + 1;
         h.steps[slot] = t;
-        const double lr = h.lr_dev ? (double)*h.lr_dev : h.lr;
-        float* s = h.scal + 8 * (size_t)slot;
-        s[0] = (float)(1.0 - lr * h.wd);
-        s[1] = (float)(lr / (1.0 - int_pow(h.b1, t)));
-        s[2] = (float)(1.0 / sqrt(1.0 - int_pow(h.b2, t)));
-        s[3] = __uint_as_float((uint32_t)t * DITHER_M);
-        s[4] = __uint_as_float((uint32_t)t * DITHER_V);
+        *(MtScal*)(h.scal + 8 * (size_t)slot) = step_numbers(h, t);
     }
+}
+// A small step without a norm has no such launch: every workgroup works the numbers out for itself.  The count may advance once all
+// of the tensor's workgroups have read it: they are counted (word 7 of the slot's scalars), and the last one writes it.
+__device__ __forceinline__ MtScal own_numbers(const MtPrep& h, uint32_t slot, uint32_t chunks) {
+    __shared__ MtScal shared;
+    if (threadIdx.x == 0) {
+        const long t = h.steps[slot] + 1;
+        asm volatile("" ::"v"((uint32_t)t), "v"((uint32_t)(t >> 32)) : "memory");      // the count has arrived
+        uint32_t* seen = (uint32_t*)h.scal + 8 * (size_t)slot + 7;
+        if (__hip_atomic_fetch_add(seen, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == chunks - 1) {
+            h.steps[slot] = t;
+            *seen = 0;
+        }
+        shared = step_numbers(h, t);
+    }
+    __syncthreads();
+    const MtScal s = shared;
+    __syncthreads();
+    return s;
 }
 
 // workgroups 0..nsum-1: partial sums; with PREP one more, which prepares the step of the same tensors
@@ -565,7 +592,7 @@ __device__ __forceinline__ void adamw_chunk(const MtJob& jb, const MtHyper& h, c
 }
 
 template <bool S8, bool NT>
-__global__ __launch_bounds__(256) void multi_adamw_kernel(const MtTable tab, const MtHyper h, const MtClip clip) {
+__global__ __launch_bounds__(256) void multi_adamw_kernel(const MtTable tab, const MtHyper h, const MtClip clip, const MtPrep own) {
     const MtFind find(tab);
     const float coef = clip_coef(clip);
     for (uint32_t w = blockIdx.x; w < tab.nchunk; w += gridDim.x) {
@@ -573,8 +600,8 @@ __global__ __launch_bounds__(256) void multi_adamw_kernel(const MtTable tab, con
         const int j = find(c);
         const MtJob& jb = tab.job[j];
         const long c0 = (long)(c - tab.first[j]) * MT_CHUNK;
-        const float* sc = h.scal + 8 * (size_t)(jb.slot_flags >> 2);
-        const MtScal s = {sc[0], sc[1], sc[2], __float_as_uint(sc[3]), __float_as_uint(sc[4])};
+        const uint32_t slot = jb.slot_flags >> 2;
+        const MtScal s = own.steps ? own_numbers(own, slot, mt_chunks(jb.n)) : *(const MtScal*)(h.scal + 8 * (size_t)slot);
         switch (jb.slot_flags & 3) {
             case 0: adamw_chunk<false, false, S8, NT>(jb, h, s, coef, c0); break;
             case VAE_MT_GRAD_BF16: adamw_chunk<false, true, S8, NT>(jb, h, s, coef, c0); break;
@@ -702,8 +729,9 @@ static int check_tensors(const char* who, const vae_mt_tensor* t, int count, boo
     return 0;
 }
 
-// the next launch's table, from tensor `at` on; returns the tensor after its last.  Empty tensors keep their slot (their step counts
-// on) but have no chunk: their first chunk is the next tensor's, which find() then prefers.
+// the next launch's table, from tensor `at` on; returns the tensor after its last.  A tensor without a chunk has the next one's as its
+// first, and find() takes the last of them.
+// chunk: elements, or 0: the step's (mt_chunks)
 static int fill_table(const vae_mt_tensor* t, int count, int at, int chunk, MtTable& tab) {
     tab.count = 0;
     tab.nchunk = 0;
@@ -711,7 +739,7 @@ static int fill_table(const vae_mt_tensor* t, int count, int at, int chunk, MtTa
         const int k = tab.count++;
         tab.first[k] = tab.nchunk;
         tab.job[k] = {t[at].param, t[at].grad, t[at].n, t[at].block, t[at].slot << 2 | t[at].flags};
-        tab.nchunk += (uint32_t)((t[at].n + chunk - 1) / chunk);
+        tab.nchunk += chunk ? (uint32_t)((t[at].n + chunk - 1) / chunk) : mt_chunks(t[at].n);
     }
     for (int k = tab.count; k < MT_TENSORS; ++k) tab.first[k] = 0xFFFFFFFFu;
     return at;
@@ -743,13 +771,14 @@ static double step_bytes(const MtTable& t, bool eight) {
 }
 static int update_grid(uint32_t nchunk) { return nchunk < AD_GRID ? (int)nchunk : (int)AD_GRID; }
 
-// sum-of-squares launches over a list (with `prep`: the step is prepared by the same launches); adds their partial sums to *np
-static int sumsq_list(const vae_mt_tensor* t, int count, long all_chunks, const MtPrep* prep, bool sums, double* partial, int* np, hipStream_t s) {
+// sum-of-squares launches over a list (with `prep`: the step is prepared by the same launches; without `partial`: that alone); adds
+// the number of their partial sums to *np
+static int sumsq_list(const vae_mt_tensor* t, int count, long all_chunks, const MtPrep* prep, double* partial, int* np, hipStream_t s) {
     MtTable tab;
     for (int at = 0; at < count;) {
         at = fill_table(t, count, at, SQ_CHUNK, tab);
         int n = 0;
-        if (sums && tab.nchunk) {
+        if (partial && tab.nchunk) {
             // of a list longer than one launch each launch gets its share of the partial sums, and at least one
             n = (int)((double)MT_PARTIALS * tab.nchunk / (double)all_chunks);
             if (n < 1) n = 1;
@@ -781,7 +810,7 @@ extern "C" int vae_multi_grad_norm(const vae_mt_tensor* tensors, int count, doub
     VAE_CHECK(partial && norm_out, "vae_multi_grad_norm: null pointer");
     hipStream_t s = (hipStream_t)stream;
     int np = 0;
-    if (int rc = sumsq_list(tensors, count, chunks, nullptr, true, partial, &np, s)) return rc;
+    if (int rc = sumsq_list(tensors, count, chunks, nullptr, partial, &np, s)) return rc;
     const MtClip clip = {partial, np ? np : -1, grad_mul, -1.f, norm_out};
     hipLaunchKernelGGL(multi_norm_kernel, dim3(1), dim3(64), 0, s, clip);
     VAE_LAUNCH_CHECK("multi_norm_kernel");
@@ -797,7 +826,7 @@ extern "C" int vae_multi_clip(const vae_mt_tensor* tensors, int count, double* p
     hipStream_t s = (hipStream_t)stream;
     const bool nt = grad_bytes(tensors, count) > MT_STREAM_BYTES;
     int np = 0;
-    if (int rc = sumsq_list(tensors, count, chunks, nullptr, true, partial, &np, s)) return rc;
+    if (int rc = sumsq_list(tensors, count, chunks, nullptr, partial, &np, s)) return rc;
     MtTable tab;
     for (int at = 0; at < count;) {
         at = fill_table(tensors, count, at, MT_CHUNK, tab);
@@ -812,6 +841,8 @@ extern "C" int vae_multi_clip(const vae_mt_tensor* tensors, int count, double* p
     }
     return 0;
 }
+
+static MtPrep prep_of(const vae_mt_group& q) { return {q.steps, q.scalars, q.lr_dev, q.lr, q.beta1, q.beta2, q.weight_decay}; }
 
 extern "C" int vae_multi_adamw_step(const vae_mt_group* groups, int ngroups, double* partial, float grad_mul, float max_norm, float* norm_out,
                                     void* stream) {
@@ -842,19 +873,21 @@ extern "C" int vae_multi_adamw_step(const vae_mt_group* groups, int ngroups, dou
     hipStream_t s = (hipStream_t)stream;
     // what the step holds in memory, all groups together
     double bytes = 0.0;
+    long step_chunks = 0;
     for (int k = 0; k < ngroups; ++k)
         for (int i = 0; i < groups[k].count; ++i) {
             const vae_mt_tensor& t = groups[k].tensors[i];
+            step_chunks += mt_chunks(t.n);
             bytes += (double)t.n * ((t.flags & VAE_MT_GRAD_BF16 ? 2 : 4) + 4 + (groups[k].state_bits == 8 ? 2 : 8));
         }
     const bool nt = bytes > MT_STREAM_BYTES;
     int np = 0;
-    for (int k = 0; k < ngroups; ++k) {
-        const vae_mt_group& q = groups[k];
-        const MtPrep prep = {q.steps, q.scalars, q.lr_dev, q.lr, q.beta1, q.beta2, q.weight_decay};
-        if (int rc = sumsq_list(q.tensors, q.count, all, &prep, sums, partial, &np, s)) return rc;
+    const bool norm = sums && all > 0, own = !norm && step_chunks <= MT_OWN_CHUNKS;
+    for (int k = 0; k < ngroups && !own; ++k) {
+        const MtPrep prep = prep_of(groups[k]);
+        if (int rc = sumsq_list(groups[k].tensors, groups[k].count, all, &prep, norm ? partial : nullptr, &np, s)) return rc;
     }
-    if (all == 0 && norm_out) {      // nothing but empty tensors: no launch below writes the norm
+    if (!norm && norm_out) {      // nothing but empty tensors: no launch below writes the norm
         hipLaunchKernelGGL(multi_norm_kernel, dim3(1), dim3(64), 0, s, MtClip{partial, -1, grad_mul, -1.f, norm_out});
         VAE_LAUNCH_CHECK("multi_norm_kernel");
     }
@@ -864,16 +897,17 @@ extern "C" int vae_multi_adamw_step(const vae_mt_group* groups, int ngroups, dou
         const MtHyper h = {q.exp_avg, q.exp_avg_sq, (short2*)q.bases, q.remainder, q.scalars, (float)q.beta1, (float)(1.0 - q.beta1), (float)q.beta2,
                            (float)(1.0 - q.beta2), (float)q.eps};
         for (int at = 0; at < q.count;) {
-            at = fill_table(q.tensors, q.count, at, MT_CHUNK, tab);
+            at = fill_table(q.tensors, q.count, at, 0, tab);
             if (!tab.nchunk) continue;
             const MtClip clip = {partial, np, grad_mul, max_norm, norm_out};
+            const MtPrep numbers = own ? prep_of(q) : MtPrep{};
             const int grid = update_grid(tab.nchunk);
             const bool eight = q.state_bits == 8;
             ProfScope prof(eight ? "multi_adamw8_kernel" : "multi_adamw_kernel", 0.0, step_bytes(tab, eight), s);
-            if (eight && nt) hipLaunchKernelGGL((multi_adamw_kernel<true, true>), dim3(grid), dim3(256), 0, s, tab, h, clip);
-            else if (eight) hipLaunchKernelGGL((multi_adamw_kernel<true, false>), dim3(grid), dim3(256), 0, s, tab, h, clip);
-            else if (nt) hipLaunchKernelGGL((multi_adamw_kernel<false, true>), dim3(grid), dim3(256), 0, s, tab, h, clip);
-            else hipLaunchKernelGGL((multi_adamw_kernel<false, false>), dim3(grid), dim3(256), 0, s, tab, h, clip);
+            if (eight && nt) hipLaunchKernelGGL((multi_adamw_kernel<true, true>), dim3(grid), dim3(256), 0, s, tab, h, clip, numbers);
+            else if (eight) hipLaunchKernelGGL((multi_adamw_kernel<true, false>), dim3(grid), dim3(256), 0, s, tab, h, clip, numbers);
+            else if (nt) hipLaunchKernelGGL((multi_adamw_kernel<false, true>), dim3(grid), dim3(256), 0, s, tab, h, clip, numbers);
+            else hipLaunchKernelGGL((multi_adamw_kernel<false, false>), dim3(grid), dim3(256), 0, s, tab, h, clip, numbers);
             VAE_LAUNCH_CHECK("multi_adamw_kernel");
         }
     }

@@ -296,6 +296,23 @@ def test_a_group_added_later_and_a_scheduler(O):
     assert len(opt.param_groups) == 2
 
 
+def test_hooks_and_a_list_that_was_changed(O):
+    p, seen = torch.nn.Parameter(torch.ones(300, device=DEV)), []
+    opt = O.MultiAdamW([p], lr=0.1)
+    pre = opt.register_step_pre_hook(lambda o, args, kw: seen.append(("pre", o is opt, args[0] is opt, kw["max_norm"])))
+    post = opt.register_step_post_hook(lambda o, args, kw: seen.append(("post", o is opt)))
+    p.grad = torch.ones_like(p)
+    opt.step(max_norm=2.0)
+    assert seen == [("pre", True, True, 2.0), ("post", True)]
+    pre.remove(), post.remove()
+    opt.register_step_pre_hook(lambda o, args, kw: (args, {"max_norm": 0.0}))       # a clip to nothing
+    opt.step(max_norm=2.0)
+    assert float(opt.grad_norm) > 0 and len(seen) == 2
+    opt.param_groups[0]["params"].append(torch.nn.Parameter(torch.ones(5, device=DEV)))
+    with pytest.raises(RuntimeError, match="list of tensors was changed"):
+        opt.step()
+
+
 @pytest.mark.parametrize("what", ["nan", "inf"])
 @pytest.mark.parametrize("bits", [32, 8])
 def test_a_bad_gradient_stays_in_its_element(O, what, bits):

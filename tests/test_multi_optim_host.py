@@ -66,7 +66,8 @@ def test_norm_and_clip_refuse_scratch_and_counts():
     ([job()], dict(state_bits=16), "state_bits"), ([job()], dict(beta1=1.0), "betas"), ([job()], dict(beta2=-0.1), "betas"),
     ([job()], dict(eps=-1.0), "eps"), ([job()], dict(state_bits=8, eps=1e-13, bases=4096), "8-bit moments need"), ([job()], dict(lr=-1.0), "lr"), ([job()], dict(weight_decay=float("nan")), "weight_decay"),
     ([job()], dict(exp_avg=None), "null state"), ([job()], dict(state_bits=8), "null state"), ([job()], dict(exp_avg=4100), "16-byte"),
-    ([job()], dict(steps=None), "step counts"), ([job(n=1025)], {}, "reaches behind"), ([job(block=4)], {}, "reaches behind"),
+    ([job()], dict(steps=None), "step counts"), ([job()], dict(steps=4100), "not aligned"), ([job()], dict(lr_dev=4098), "not aligned"),
+    ([job()], dict(nslots=65537), "nslots"), ([job()], dict(nslots=-1), "nslots"), ([job(n=1025)], {}, "reaches behind"), ([job(block=4)], {}, "reaches behind"),
     ([job(slot=1)], {}, "slot"), ([job(param=None)], {}, "parameter is null"), ([job(param=4098)], {}, "not aligned"),
     ([job(flags=1)], {}, "remainder"), ([job()], dict(struct_size=8), "struct_size")])
 def test_step_refuses(jobs, kw, match):

@@ -860,8 +860,10 @@ extern "C" int vae_multi_adamw_step(const vae_mt_group* groups, int ngroups, dou
         VAE_CHECK(q.state_bits == 32 || q.eps >= VAE_MT_MIN_EPS8, "vae_multi_adamw_step: eps=%g: 8-bit moments need at least %g", q.eps, VAE_MT_MIN_EPS8);
         VAE_CHECK(q.eps >= 0.0 && q.weight_decay >= 0.0 && (q.lr_dev || q.lr >= 0.0), "vae_multi_adamw_step: lr=%g, eps=%g and weight_decay=%g must not be negative",
                   q.lr, q.eps, q.weight_decay);
+        VAE_CHECK(q.nslots >= 0 && q.nslots <= VAE_MT_MAX_TENSORS, "vae_multi_adamw_step: nslots=%d out of range (0..%d)", q.nslots, VAE_MT_MAX_TENSORS);
         long chunks = 0;
         if (check_tensors("vae_multi_adamw_step", q.tensors, q.count, true, true, q.nblocks, q.nslots, &chunks)) return 1;
+        VAE_CHECK(((uintptr_t)q.steps & 7) == 0 && ((uintptr_t)q.lr_dev & 3) == 0, "vae_multi_adamw_step: steps or lr_dev not aligned to its type");
         VAE_CHECK(q.count == 0 || (q.steps && q.scalars), "vae_multi_adamw_step: null step counts or scalars");
         VAE_CHECK(chunks == 0 || (q.exp_avg && q.exp_avg_sq && (q.state_bits == 32 || q.bases)), "vae_multi_adamw_step: null state");
         VAE_CHECK((((uintptr_t)q.exp_avg | (uintptr_t)q.exp_avg_sq | (uintptr_t)q.remainder | (uintptr_t)q.bases | (uintptr_t)q.scalars) & 15) == 0,

@@ -177,8 +177,9 @@ class _GroupState:
     the library."""
 
     def __init__(self, params, state_bits):
-        self.params = params
+        self.params = list(params)
         self.device = params[0].device
+        self.home = _lib.current_stream()
         self.bits = state_bits
         self.shapes = [tuple(p.shape) for p in params]
         self.strides = [p.stride() for p in params]
@@ -208,8 +209,13 @@ class _GroupState:
                               exp_avg_sq=self.exp_avg_sq.data_ptr(), bases=_lib.ptr(self.bases), remainder=_lib.ptr(self.remainder),
                               nblocks=self.nblocks, steps=self.steps.data_ptr(), scalars=self.scalars.data_ptr())
 
-    def buffers(self):
-        return [b for b in (self.exp_avg, self.exp_avg_sq, self.bases, self.remainder, self.steps, self.scalars) if b is not None]
+    def used_on(self, stream):
+        """the allocator may not hand the state on before this stream's work on it is done"""
+        if stream != self.home:
+            cur = torch.cuda.current_stream()
+            for b in (self.exp_avg, self.exp_avg_sq, self.bases, self.remainder, self.steps, self.scalars):
+                if b is not None:
+                    b.record_stream(cur)
 
     def check_param(self, k):
         """a parameter is read and written through its address: it still has to be what the state was laid out for"""
@@ -275,11 +281,11 @@ class MultiAdamW(torch.optim.Optimizer):
     moments), parameters without a gradient left alone.  All arithmetic is in 32 bits; step counts live on the device.
 
     ``state_bits=8`` (also per group) holds both moments in 8 bits, 2 bytes a parameter instead of 8: blocks of 256 elements, 8 levels per
-    octave, rounded with a dither that is unbiased over the steps.  A bf16 parameter keeps a 16-bit remainder with which it is a
+    octave, rounded with a dither over the steps (see csrc/multi_optim.hip).  A bf16 parameter keeps a 16-bit remainder with which it is a
     32-bit master; writing the parameter from outside needs nothing.
 
     ``step(max_norm=1.0)`` is ``clip_grad_norm_(params, 1.0); step()`` without the pass that rewrites the gradients: two launches
-    per group and 192 tensors; the norm before the clip is in ``grad_norm``.  Gradients are multiplied by ``grad_mul`` first
+    per group and 192 tensors (a small step without a clip: one); the norm before the clip is in ``grad_norm``.  Gradients are multiplied by ``grad_mul`` first
     (1/world_size after a SUM all-reduce).
 
     A step can be captured into a graph: step counts advance when it is replayed.  A float ``lr`` is recorded as it is; give an fp32
@@ -361,11 +367,11 @@ class MultiAdamW(torch.optim.Optimizer):
     def step(self, closure=None, max_norm=None):
         """One step; with ``max_norm`` the gradients' global norm (over all groups) is clipped to it first.  ``closure``, as in torch,
         recomputes the loss and its gradients; its value is returned."""
+        args, kwargs = (self, closure), {"max_norm": max_norm}
         if _global_pre_hooks or self._optimizer_step_pre_hooks:
             for hook in (*_global_pre_hooks.values(), *self._optimizer_step_pre_hooks.values()):
-                changed = hook(self, (closure,), {"max_norm": max_norm})
-                if changed is not None:
-                    (closure,), max_norm = changed[0], changed[1].get("max_norm")
+                args, kwargs = hook(self, args, kwargs) or (args, kwargs)
+            closure, max_norm = args[1] if len(args) > 1 else kwargs.get("closure"), kwargs.get("max_norm")
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -373,7 +379,7 @@ class MultiAdamW(torch.optim.Optimizer):
         self._step(max_norm)
         if _global_post_hooks or self._optimizer_step_post_hooks:
             for hook in (*self._optimizer_step_post_hooks.values(), *_global_post_hooks.values()):
-                hook(self, (closure,), {"max_norm": max_norm})
+                hook(self, args, kwargs)
         return loss
 
     step.hooked = True      # torch would wrap it into a profiler range, 14 us of host time a step
@@ -394,6 +400,8 @@ class MultiAdamW(torch.optim.Optimizer):
             total += n
             keep.append(kept)
             c, lr = st.c, g["lr"]
+            if isinstance(lr, torch.Tensor) and lr.device != st.device:
+                raise RuntimeError(f"MultiAdamW: lr lives on {lr.device}, the parameters on {st.device}")
             c.lr, c.lr_dev = (0.0, lr.data_ptr()) if isinstance(lr, torch.Tensor) else (float(lr), None)
             (c.beta1, c.beta2), c.eps, c.weight_decay = g["betas"], g["eps"], g["weight_decay"]
             self._c[k] = c
@@ -402,13 +410,12 @@ class MultiAdamW(torch.optim.Optimizer):
                 self.grad_norm.zero_()
             return
         stream = _lib.current_stream()
-        if stream != self._home:
-            cur = torch.cuda.current_stream()
+        if stream != self._home or len(self._groups) > 1:
             for st in self._groups:
-                for b in st.buffers():
-                    b.record_stream(cur)
-            self._partial.record_stream(cur)
-            self.grad_norm.record_stream(cur)
+                st.used_on(stream)
+        if stream != self._home:
+            self._partial.record_stream(torch.cuda.current_stream())
+            self.grad_norm.record_stream(torch.cuda.current_stream())
         _lib.call("vae_multi_adamw_step", ctypes.byref(self._c), len(self._groups), self._partial.data_ptr(), float(self.grad_mul), clip,
                   self.grad_norm.data_ptr() if clip >= 0.0 else None, stream)
 
@@ -420,6 +427,7 @@ class MultiAdamW(torch.optim.Optimizer):
         if st.bits == 32:
             return st.exp_avg, st.exp_avg_sq
         _lib.check_device(st.exp_avg)
+        st.used_on(_lib.current_stream())
         m, v = (torch.empty(st.exp_avg.numel(), dtype=torch.bfloat16, device=st.device) for _ in range(2))
         self._unpack(st, st.exp_avg, st.exp_avg_sq, st.bases, m, v)
         return m, v
@@ -433,6 +441,7 @@ class MultiAdamW(torch.optim.Optimizer):
         """32-bit values of a group's parameters in the state's layout: a bf16 parameter's master, an fp32 parameter itself"""
         st = self._groups[group]
         _lib.check_device(st.exp_avg)
+        st.used_on(_lib.current_stream())
         # every block is some tensor's and is written whole
         out = (torch.empty if st.nblocks else torch.zeros)(max(st.nblocks, 1) * _lib.MT_BLOCK, device=st.device)
         jobs = _tables.room(len(st.params))

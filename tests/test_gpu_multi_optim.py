@@ -209,6 +209,62 @@ def test_three_steps(O, sizes, pd, gd, shift, bits):
     assert total == sum(p.numel() for p in ps)
 
 
+@pytest.mark.parametrize("sizes", list(SIZES))
+@pytest.mark.parametrize("bits", [32, 8])
+def test_with_and_without_a_norm_the_step_is_the_same(O, sizes, bits):
+    """a norm that clips nothing changes no bit: the numbers prepared beside the norm, those worked out by every workgroup of a small step and
+    those of a launch of their own agree, and the counts advance alike"""
+    n = SIZES[sizes]
+    vals, _, _ = tensors(n, F32, 0, 3, 0.05)
+    ps, qs = [torch.nn.Parameter(v.clone()) for v in vals], [torch.nn.Parameter(v.clone()) for v in vals]
+    a, b = O.MultiAdamW(ps, lr=1e-3, state_bits=bits), O.MultiAdamW(qs, lr=1e-3, state_bits=bits)
+    for t in range(5):
+        gs, _, _ = tensors(n, F32, 0, 30 + t, 0.3)
+        for k, (p, q, g) in enumerate(zip(ps, qs, gs)):
+            p.grad = q.grad = None if (k + t) % 3 == 0 and len(n) > 1 else g
+        a.step()
+        b.step(max_norm=1e30)
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs)), t
+    assert all(torch.equal(x, y) for x, y in zip(a.flat_moments(), b.flat_moments()))
+    sa, sb = a.state_dict()["state"], b.state_dict()["state"]
+    want = [sum(not ((k + t) % 3 == 0 and len(n) > 1) for t in range(5)) for k in range(len(n))]
+    assert [float(sa[k]["step"]) for k in range(len(n))] == want == [float(sb[k]["step"]) for k in range(len(n))]
+
+
+def test_two_optimizers_at_once(O):
+    """two threads, each with its own model, optimizer and stream, against the same steps one after the other"""
+    import threading
+    n = [5000, 300, 70_000, 1]
+
+    def make(seed):
+        vals, _, _ = tensors(n, F32, 0, seed, 0.05)
+        ps = [torch.nn.Parameter(v) for v in vals]
+        return ps, O.MultiAdamW(ps, lr=1e-3, state_bits=8), [tensors(n, F32, 0, 1000 * seed + t, 0.3)[0] for t in range(20)]
+
+    def run(ps, opt, grads, out):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for g in grads:
+                for p, x in zip(ps, g):
+                    p.grad = x.clone()
+                out.append(O.clip_grad_norm_(ps, 1.0))
+                opt.step(max_norm=0.5)
+        torch.cuda.current_stream().synchronize()
+    both, alone = [make(1), make(2)], [make(1), make(2)]
+    torch.cuda.synchronize()
+    norms = [[] for _ in range(4)]
+    threads = [threading.Thread(target=run, args=(*x, norms[k])) for k, x in enumerate(both)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for k, x in enumerate(alone):
+        run(*x, norms[2 + k])
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert all(torch.equal(p, q) for p, q in zip(both[k][0], alone[k][0]))
+        assert all(torch.equal(x, y) for x, y in zip(norms[k], norms[2 + k])) and len(norms[k]) == 20
+
+
 def test_bf16_parameters_follow_the_fp32_run_to_the_bit(O):
     """parameter and remainder are 32 bits of master: the run is that of fp32 parameters with the same start and gradients"""
     n = [300, 4097, 1]

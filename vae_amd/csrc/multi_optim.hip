@@ -408,11 +408,12 @@ __device__ __forceinline__ void split_master(float w, bf16_t& p, short& r) {
 // One block of 256 elements of one tensor, a wave's work: 4 elements a lane.  All of a wave's blocks of a chunk are loaded before the
 // first is stored: the stores could alias the later loads as far as the compiler knows, and would wait for one another.
 // Bound by HBM: 28 bytes a parameter in fp32 with 32-bit moments, 16 with 8-bit ones (26 and 14 in bf16 with remainder).
-// 69.8 M fp32 parameters in 88 tensors: 341 us, 5.7 TB/s; 8-bit moments 192 us, 5.8 TB/s (a pass over one array in place
-// reaches 5.9).  20 M bf16 parameters in 217 tensors off their alignment: 86 us, 6.0 TB/s.
+// 69.8 M fp32 parameters in 88 tensors: 336 us, 5.8 TB/s (295 with the gradients still cached from the norm); 8-bit moments
+// 182 us, 6.1 TB/s (a pass over one array in place reaches 5.9).  20 M bf16 parameters in 217 tensors off their alignment: 91 us,
+// 5.7 TB/s.
 //
 // In 8 bits the vector instructions count: 16 bytes a parameter at 5.9 TB/s leave about 100 of them.  The first form took
-// 110 a parameter and 240 us, this one 66 (bf16: 81).  So
+// 110 a parameter and 240 us, this one 65 (bf16: 77).  So
 // - root and reciprocal are the hardware's, 1 ulp each, of a step that is itself a small part of the parameter.  The hardware takes
 //   the root of a subnormal for 0, which nobody sees next to an eps of at least 1e-12 (VAE_MT_MIN_EPS8): smaller ones are refused;
 // - values that are not finite, their codes, and fp32's last level are looked after in branches that a wave seldom takes;

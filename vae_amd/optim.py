@@ -466,13 +466,14 @@ class MultiAdamW(torch.optim.Optimizer):
         state, groups, at = {}, [], 0
         for g, st in zip(self.param_groups, self._groups):
             steps = st.steps.tolist()
+            bases = st.bases.t().contiguous().int() if st.bits == 8 else None
             for k in range(len(st.params)):
                 e = {"step": torch.tensor(float(steps[k]), dtype=torch.float32 if steps[k] < 1 << 24 else torch.float64)}
                 if st.bits == 32:
                     e["exp_avg"], e["exp_avg_sq"] = st.view(st.exp_avg, k), st.view(st.exp_avg_sq, k)
                 else:
                     e["exp_avg_q"], e["exp_avg_sq_q"] = st.run(st.exp_avg, k), st.run(st.exp_avg_sq, k)
-                    e["exp_avg_base"], e["exp_avg_sq_base"] = (st.bases[st.rows(k), j].int() for j in (0, 1))
+                    e["exp_avg_base"], e["exp_avg_sq_base"] = (bases[j, st.rows(k)] for j in (0, 1))
                     e["stride"] = st.strides[k]
                 if st.dtypes[k] is torch.bfloat16:
                     e["remainder"] = st.view(st.remainder, k)
@@ -534,8 +535,9 @@ class MultiAdamW(torch.optim.Optimizer):
             raise ValueError(f"MultiAdamW: the step count of parameter {k} is {step}")
         if ("exp_avg" in e) != ("exp_avg_sq" in e) or ("exp_avg" in e and "exp_avg_q" in e):
             raise ValueError(f"MultiAdamW: the entry of parameter {k} has {sorted(e)}")
-        for key in ("exp_avg", "exp_avg_sq", "exp_avg_q", "exp_avg_sq_q", "remainder"):
-            fits(key, st.n[k])
+        for key in e:
+            if key in ("exp_avg", "exp_avg_sq", "exp_avg_q", "exp_avg_sq_q", "remainder"):
+                fits(key, st.n[k])
         if "exp_avg_q" in e:
             for key in ("exp_avg_sq_q", "exp_avg_base", "exp_avg_sq_base"):
                 if key not in e:
@@ -574,7 +576,9 @@ class MultiAdamW(torch.optim.Optimizer):
             q, bases = scratch(torch.uint8), torch.zeros(max(st.nblocks, 1), 2, dtype=torch.int16, device=st.device)
         if eight:
             fill(q, st.run, eight, ("exp_avg_q", "exp_avg_sq_q"))
-            rows = torch.cat([torch.arange(st.rows(k).start, st.rows(k).stop) for k in eight]).to(st.device)
+            rows = slice(0, st.nblocks)
+            if len(eight) < len(row):
+                rows = torch.cat([torch.arange(st.rows(k).start, st.rows(k).stop) for k in eight]).to(st.device)
             for j, key in enumerate(("exp_avg_base", "exp_avg_sq_base")):
                 bases[rows, j] = torch.cat([row[k][key].reshape(-1) for k in eight]).to(device=st.device, dtype=torch.int16)
         if st.bits == 32:

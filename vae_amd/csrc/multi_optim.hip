@@ -35,7 +35,7 @@
 
 namespace vae {
 
-#define MT_TENSORS 192           // tensors one launch takes: 32 + 4 bytes of kernel arguments each
+#define MT_TENSORS 256           // tensors one launch takes: 32 + 4 bytes of kernel arguments each
 #define MT_CHUNK 4096            // elements a workgroup takes at a time
 #define AD_DEEP 4                // blocks a wave of the step has in flight
 #define MT_BLOCK 256             // elements of one tensor that share a base; a wave's 64 lanes x 4
@@ -745,6 +745,8 @@ static int fill_table(const vae_mt_tensor* t, int count, int at, int chunk, MtTa
     for (int k = tab.count; k < MT_TENSORS; ++k) tab.first[k] = 0xFFFFFFFFu;
     return at;
 }
+// the first tensor of a list's last launch; negative: there is none
+static int last_table(int count) { return count > 0 ? (count - 1) / MT_TENSORS * MT_TENSORS : -1; }
 static double elem_bytes(const MtTable& t, int per_grad_f32) {
     double b = 0;
     for (int k = 0; k < t.count; ++k) b += (double)t.job[k].n * ((t.job[k].slot_flags & VAE_MT_GRAD_BF16) ? per_grad_f32 / 2 : per_grad_f32);
@@ -802,7 +804,7 @@ static int sumsq_list(const vae_mt_tensor* t, int count, long all_chunks, const 
 using namespace vae;
 
 extern "C" int vae_multi_partials(int count) {
-    return MT_PARTIALS + (count < 0 ? 0 : count) / MT_TENSORS + 1 + VAE_MT_MAX_GROUPS;
+    return MT_PARTIALS + (count < 0 ? 0 : count) / (MT_TENSORS / 2) + 1 + VAE_MT_MAX_GROUPS;      // more than there are launches
 }
 
 extern "C" int vae_multi_grad_norm(const vae_mt_tensor* tensors, int count, double* partial, float grad_mul, float* norm_out, void* stream) {
@@ -829,8 +831,8 @@ extern "C" int vae_multi_clip(const vae_mt_tensor* tensors, int count, double* p
     int np = 0;
     if (int rc = sumsq_list(tensors, count, chunks, nullptr, partial, &np, s)) return rc;
     MtTable tab;
-    for (int at = 0; at < count;) {
-        at = fill_table(tensors, count, at, MT_CHUNK, tab);
+    for (int at = last_table(count); at >= 0; at -= MT_TENSORS) {
+        fill_table(tensors, count, at, MT_CHUNK, tab);
         if (!tab.nchunk) continue;
         const MtClip clip = {partial, np, grad_mul, max_norm, norm_out};
         {
@@ -895,12 +897,12 @@ extern "C" int vae_multi_adamw_step(const vae_mt_group* groups, int ngroups, dou
         VAE_LAUNCH_CHECK("multi_norm_kernel");
     }
     MtTable tab;
-    for (int k = 0; k < ngroups; ++k) {
+    for (int k = ngroups - 1; k >= 0; --k) {       // from the last launch to the first, as within a launch
         const vae_mt_group& q = groups[k];
         const MtHyper h = {q.exp_avg, q.exp_avg_sq, (short2*)q.bases, q.remainder, q.scalars, (float)q.beta1, (float)(1.0 - q.beta1), (float)q.beta2,
                            (float)(1.0 - q.beta2), (float)q.eps};
-        for (int at = 0; at < q.count;) {
-            at = fill_table(q.tensors, q.count, at, 0, tab);
+        for (int at = last_table(q.count); at >= 0; at -= MT_TENSORS) {
+            fill_table(q.tensors, q.count, at, 0, tab);
             if (!tab.nchunk) continue;
             const MtClip clip = {partial, np, grad_mul, max_norm, norm_out};
             const MtPrep numbers = own ? prep_of(q) : MtPrep{};

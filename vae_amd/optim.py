@@ -138,7 +138,7 @@ def _grad_jobs_general(params, first, who, write):
 
 
 def grad_norm(parameters):
-    """Global L2 norm of the parameters' gradients as a 0-dim fp32 tensor: one launch per 192 tensors and one that finishes the
+    """Global L2 norm of the parameters' gradients as a 0-dim fp32 tensor: one launch per 256 tensors and one that finishes the
     sum.  Squares and sums in 64 bits, in a fixed order."""
     jobs, n, keep = _grad_jobs(parameters, "grad_norm", False)
     if n == 0:
@@ -152,7 +152,7 @@ def grad_norm(parameters):
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """torch.nn.utils.clip_grad_norm_ (vae/training/train.py:336) for fp32 and bf16 gradients of any number of tensors: scales
     them in place by ``min(1, max_norm / (norm + 1e-6))`` and returns the norm before that as a 0-dim fp32 tensor.  Two launches per
-    192 tensors, no host synchronisation unless ``error_if_nonfinite``."""
+    256 tensors, no host synchronisation unless ``error_if_nonfinite``."""
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"clip_grad_norm_: max_norm={max_norm} must not be negative or NaN")
@@ -285,7 +285,7 @@ class MultiAdamW(torch.optim.Optimizer):
     32-bit master; writing the parameter from outside needs nothing.
 
     ``step(max_norm=1.0)`` is ``clip_grad_norm_(params, 1.0); step()`` without the pass that rewrites the gradients: two launches
-    per group and 192 tensors (a small step without a clip: one); the norm before the clip is in ``grad_norm``.  Gradients are multiplied by ``grad_mul`` first
+    per group and 256 tensors (a small step without a clip: one); the norm before the clip is in ``grad_norm``.  Gradients are multiplied by ``grad_mul`` first
     (1/world_size after a SUM all-reduce).
 
     A step can be captured into a graph: step counts advance when it is replayed.  A float ``lr`` is recorded as it is; give an fp32

@@ -305,8 +305,13 @@ struct MtClip {
 // gradient NaN and an infinite one makes them 0 or NaN, as torch's clip_grad_norm_ does.
 __device__ __forceinline__ float clip_coef(const MtClip& c) {
     if (c.npartial == 0) return c.grad_mul;
-    double a = 0.0;
-    for (int i = threadIdx.x & 63; i < c.npartial; i += 64) a += c.partial[i];
+    const int lane = threadIdx.x & 63;
+    double v[MT_PARTIALS / 64], a = 0.0;
+#pragma unroll
+    for (int k = 0; k < MT_PARTIALS / 64; ++k) v[k] = lane + k * 64 < c.npartial ? c.partial[lane + k * 64] : 0.0;      // in flight together
+#pragma unroll
+    for (int k = 0; k < MT_PARTIALS / 64; ++k) a += v[k];
+    for (int i = lane + MT_PARTIALS; i < c.npartial; i += 64) a += c.partial[i];      // lists of several launches may have a few more
     a = wave_sum_d(a);
     const double norm = sqrt(a) * fabs((double)c.grad_mul);
     if (blockIdx.x == 0 && threadIdx.x == 0 && c.norm_out) *c.norm_out = (float)norm;

@@ -712,12 +712,13 @@ __global__ __launch_bounds__(256) void moments8_pack_kernel(const float* __restr
 
 // ---------------------------------------------------------------- host
 // *sq_chunks: what the norm's workgroups take in turn, over all tensors
-static int check_tensors(const char* who, const vae_mt_tensor* t, int count, bool grads, bool params, long nblocks, int nslots, long* sq_chunks) {
+static int check_tensors(const char* who, const vae_mt_tensor* t, int count, bool grads, bool params, long nblocks, long nslots, long* sq_chunks) {
     VAE_CHECK(count >= 0 && count <= VAE_MT_MAX_TENSORS && (t || count == 0), "%s: count=%d out of range (0..%d)", who, count, VAE_MT_MAX_TENSORS);
     long total = 0, sq = 0;
     for (int i = 0; i < count; ++i) {
         VAE_CHECK(t[i].n >= 0 && t[i].n < (1L << 40), "%s: tensor %d has n=%ld", who, i, t[i].n);
         VAE_CHECK((t[i].flags & ~3u) == 0, "%s: tensor %d has unknown flags 0x%x", who, i, t[i].flags);
+        VAE_CHECK(!params || (long)t[i].slot < nslots, "%s: tensor %d has slot %u of %ld", who, i, t[i].slot, nslots);      // an empty one counts its steps too
         if (t[i].n == 0) continue;
         VAE_CHECK(!grads || (t[i].grad && ((uintptr_t)t[i].grad & ((t[i].flags & VAE_MT_GRAD_BF16) ? 1 : 3)) == 0),
                   "%s: tensor %d: gradient is null or not aligned to its type", who, i);
@@ -725,7 +726,6 @@ static int check_tensors(const char* who, const vae_mt_tensor* t, int count, boo
             VAE_CHECK(t[i].param && ((uintptr_t)t[i].param & ((t[i].flags & VAE_MT_PARAM_BF16) ? 1 : 3)) == 0,
                       "%s: tensor %d: parameter is null or not aligned to its type", who, i);
             VAE_CHECK((long)t[i].block + (t[i].n + MT_BLOCK - 1) / MT_BLOCK <= nblocks, "%s: tensor %d reaches behind the state's %ld blocks", who, i, nblocks);
-            VAE_CHECK((long)t[i].slot < nslots, "%s: tensor %d has slot %u of %d", who, i, t[i].slot, nslots);
         }
         total += (t[i].n + MT_CHUNK - 1) / MT_CHUNK;
         sq += (t[i].n + SQ_CHUNK - 1) / SQ_CHUNK;
@@ -930,7 +930,7 @@ extern "C" int vae_multi_master(const vae_mt_tensor* tensors, int count, const s
     VAE_CHECK(count >= 0 && (tensors || count == 0), "vae_multi_master: count=%d", count);
     for (int i = 0; i < count; ++i)
         VAE_CHECK(!(tensors[i].flags & VAE_MT_PARAM_BF16) || tensors[i].n == 0 || remainder, "vae_multi_master: bf16 parameter %d needs the remainder buffer", i);
-    if (check_tensors("vae_multi_master", tensors, count, false, true, nblocks, 0x7FFFFFFF, &chunks)) return 1;
+    if (check_tensors("vae_multi_master", tensors, count, false, true, nblocks, 1L << 32, &chunks)) return 1;
     MtTable tab;
     for (int at = 0; at < count;) {
         at = fill_table(tensors, count, at, MT_CHUNK, tab);

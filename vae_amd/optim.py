@@ -489,9 +489,12 @@ class MultiAdamW(torch.optim.Optimizer):
         groups, state = state_dict["param_groups"], state_dict["state"]
         if [len(g["params"]) for g in groups] != [len(st.params) for st in self._groups]:
             raise ValueError("MultiAdamW: the state_dict's param groups have other lengths")
+        owned = {b.untyped_storage().data_ptr() for st in self._groups for b in (st.exp_avg, st.exp_avg_sq, st.bases, st.remainder) if b is not None}
         entries = []
         for saved, st in zip(groups, self._groups):
-            row = [state.get(i, {}) for i in saved["params"]]
+            # what state_dict() gave are views of the buffers written below: copied, because an entry may go to another tensor's place
+            row = [{key: x.clone() if isinstance(x, torch.Tensor) and x.is_cuda and x.untyped_storage().data_ptr() in owned else x
+                    for key, x in state.get(i, {}).items()} for i in saved["params"]]
             for k, e in enumerate(row):
                 self._check_entry(st, k, e)
             bases = [e[key].reshape(-1) for e in row if "exp_avg_q" in e for key in ("exp_avg_base", "exp_avg_sq_base")]

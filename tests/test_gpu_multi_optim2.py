@@ -82,3 +82,27 @@ def test_parts_of_its_own_state_dict_trade_places(O, dtype, bits):
     assert [float(a.state_dict()["state"][k]["step"]) for k in range(4)] == [3, 0, 3, 3]
     m, v = a.flat_moments()
     assert not bool(m[768:1024].any()) and not bool(v[768:1024].any()) and bool(m[:700].any()) and bool(m[1024:1724].any())
+
+
+# ------------------------------------------------------------------------------------------------ tensors exchanged or laid out anew
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_model_laid_out_anew_is_refused(O, bits):
+    """channels_last when the optimizer was made, contiguous at the step: its moments are in another order"""
+    conv = torch.nn.Conv2d(6, 8, 3).to(DEV).to(memory_format=torch.channels_last)
+    opt = O.MultiAdamW(conv.parameters(), lr=1e-2, state_bits=bits)
+    for p in conv.parameters():
+        p.grad = torch.randn_like(p)
+    opt.step()
+    was = everything(opt)
+    conv.to(memory_format=torch.contiguous_format)
+    assert conv.weight.is_contiguous()
+    kept = conv.weight.detach().clone()
+    for p in conv.parameters():
+        p.grad = torch.randn(p.shape, device=DEV)
+    for call in (lambda: opt.step(), lambda: opt.step(max_norm=1.0), opt.flat_master):
+        with pytest.raises(RuntimeError, match="make a new optimizer"):
+            call()
+    assert torch.equal(conv.weight, kept)
+    conv.to(memory_format=torch.channels_last)       # and back: it fits again
+    assert same(everything(opt), was)
+    opt.step()

@@ -15,3 +15,30 @@ def test_step_refuses_the_slot_of_an_empty_tensor(max_norm, norm, slot):
     g, arr = group([job(), job(n=0, param=None, grad=None, slot=slot)], nslots=1)
     with pytest.raises(RuntimeError, match=f"tensor 1 has slot {slot} of 1"):
         L.call("vae_multi_adamw_step", g, 1, 4096, 1.0, max_norm, norm, None)
+
+
+# ------------------------------------------------------------------------------------------------ a group's tensors (on host tensors)
+def held(monkeypatch, params, bits=32):
+    """the state of a param group, on the host"""
+    monkeypatch.setattr(L, "current_stream", lambda device=None: 0)
+    st = optim._GroupState(params, bits)
+    st.index = -1
+    return st
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_parameter_in_another_memory_order_than_its_state_is_refused(monkeypatch, bits, dtype):
+    """the state of a channels_last or transposed parameter is in that order: element k of it belongs to another element of the contiguous one"""
+    for make in (lambda: torch.randn(4, 6, 3, 3).to(dtype).to(memory_format=torch.channels_last), lambda: torch.randn(7, 5).to(dtype).t()):
+        p, q = torch.nn.Parameter(make()), torch.nn.Parameter(torch.zeros(3))
+        st = held(monkeypatch, [q, p], bits)
+        p.grad, q.grad = torch.randn_like(p), torch.zeros(3)
+        assert st.collect()[0] == 2
+        p.data = p.data.contiguous()
+        p.grad = torch.zeros(p.shape, dtype=dtype)
+        with pytest.raises(RuntimeError, match="make a new optimizer"):
+            st.collect()
+        assert L.host().collect_params(st.params, np.zeros(2, optim._JOB), st.layout, -1) == -1       # what flat_master asks first
+        p.grad = None       # without a gradient it is not stepped
+        assert st.collect()[0] == 1

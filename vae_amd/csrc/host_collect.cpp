@@ -35,9 +35,10 @@ int kind(const at::Tensor& t, int device) {
 void bump(const at::Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
 
 // collect_step(params, jobs, layout, device) -> number of tensors with a gradient, or -1 for the general way.
-// layout: int64[n][4]: elements, first block, slot, VAE_MT_* flags of the parameter the state was made for.  The parameters' version
+// layout: int64[n][4]: elements, first block, slot, VAE_MT_* flags (and STRIDED) of the parameter the state was made for.  The parameters' version
 // counters are advanced: the launch that follows writes them through their addresses.
 // collect_params: the same for all parameters, with or without a gradient, to be read only.
+constexpr int64_t STRIDED = 256;      // the state is in the order of a tensor that was not contiguous: a contiguous one is not it
 template <bool STEP>
 PyObject* collect(PyObject*, PyObject* args) {
     PyObject *list, *jobs_o, *layout_o;
@@ -63,11 +64,11 @@ PyObject* collect(PyObject*, PyObject* args) {
             const at::Tensor& g = STEP ? p.grad() : p;
             if (!g.defined()) continue;
             const int pk = kind(p, device), gk = STEP ? kind(g, device) : pk;
-            if (pk < 0 || gk < 0 || pk != (int)(row[3] & VAE_MT_PARAM_BF16) || p.numel() != row[0] || g.numel() != row[0] || !p.is_contiguous() ||
-                !g.is_contiguous() || (STEP && (p.is_inference() || p.sizes() != g.sizes())))
+            if (pk < 0 || gk < 0 || pk != (int)(row[3] & VAE_MT_PARAM_BF16) || (row[3] & STRIDED) || p.numel() != row[0] ||
+                g.numel() != row[0] || !p.is_contiguous() || !g.is_contiguous() || (STEP && (p.is_inference() || p.sizes() != g.sizes())))
                 return PyLong_FromLong(-1);
             job[live] = {const_cast<void*>(p.const_data_ptr()), g.const_data_ptr(), row[0], (unsigned)row[1], (unsigned)row[2],
-                         (unsigned)row[3] | (gk ? VAE_MT_GRAD_BF16 : 0u), 0u};
+                         (pk ? VAE_MT_PARAM_BF16 : 0u) | (gk ? VAE_MT_GRAD_BF16 : 0u), 0u};
             ++live;
             if (STEP) written.push_back(&p);
         }

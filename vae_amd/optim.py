@@ -205,6 +205,7 @@ class _GroupState:
         self.index = self.device.index
         self.param_flags = [_lib.MT_PARAM_BF16 if d is torch.bfloat16 else 0 for d in self.dtypes]
         self.layout = np.stack([self.n, self.start, np.arange(len(params)), self.param_flags], 1).astype(np.int64)
+        self.layout[:, 3] |= [0 if c else _lib.MT_STRIDED for c in self.contiguous]
         self.c = _lib.MtGroup(state_bits=state_bits, nslots=len(params), exp_avg=self.exp_avg.data_ptr(),
                               exp_avg_sq=self.exp_avg_sq.data_ptr(), bases=_lib.ptr(self.bases), remainder=_lib.ptr(self.remainder),
                               nblocks=self.nblocks, steps=self.steps.data_ptr(), scalars=self.scalars.data_ptr())

@@ -106,3 +106,26 @@ def test_a_model_laid_out_anew_is_refused(O, bits):
     conv.to(memory_format=torch.channels_last)       # and back: it fits again
     assert same(everything(opt), was)
     opt.step()
+
+
+@pytest.mark.parametrize("change", ["replaced", "exchanged", "other list"])
+def test_a_list_that_holds_other_tensors_is_refused(O, change):
+    n = [300, 300, 40]
+    ps, opt = stepped(O, n, F32, 32)
+    was, kept = everything(opt), [p.detach().clone() for p in ps]
+    group = opt.param_groups[0]
+    new = torch.nn.Parameter(ps[0].detach().clone())
+    new.grad = torch.ones_like(new)
+    if change == "replaced":
+        group["params"][0] = new
+    elif change == "exchanged":
+        group["params"][0], group["params"][1] = ps[1], ps[0]
+    else:
+        group["params"] = [*ps[:2], new]
+    for max_norm in (None, 1.0):
+        with pytest.raises(RuntimeError, match="list of tensors was changed"):
+            opt.step(max_norm=max_norm)
+    assert same(everything(opt), was) and same([p.detach() for p in ps], kept)
+    group["params"] = list(ps)
+    opt.step()
+    assert not torch.equal(ps[0], kept[0])

@@ -42,3 +42,15 @@ def test_a_parameter_in_another_memory_order_than_its_state_is_refused(monkeypat
         assert L.host().collect_params(st.params, np.zeros(2, optim._JOB), st.layout, -1) == -1       # what flat_master asks first
         p.grad = None       # without a gradient it is not stepped
         assert st.collect()[0] == 1
+
+
+def test_lists_are_compared_by_identity():
+    """a group's list as it is now against the tensors the state was made for"""
+    ps = [torch.nn.Parameter(torch.zeros(4)) for _ in range(3)]
+    same, new = L.host().same_tensors, torch.nn.Parameter(torch.zeros(4))
+    assert same(list(ps), ps) and same(ps, ps) and same([], [])
+    for now in ([ps[0], new, ps[2]], [ps[1], ps[0], ps[2]], ps[:2], [*ps, new], [], [ps[0], None, ps[2]]):
+        assert not same(now, ps)
+    assert same(tuple(ps), ps)       # any sequence will do
+    with pytest.raises(TypeError):
+        same(3, ps)

@@ -124,10 +124,24 @@ PyObject* collect_grads(PyObject*, PyObject* args) {
     }
 }
 
+// same_tensors(now, held): whether two sequences hold the same objects in the same order
+PyObject* same_tensors(PyObject*, PyObject* args) {
+    PyObject *now, *held;
+    if (!PyArg_ParseTuple(args, "OO!", &now, &PyList_Type, &held)) return nullptr;
+    PyObject* seq = PySequence_Fast(now, "same_tensors: not a sequence");
+    if (!seq) return nullptr;
+    const Py_ssize_t n = PyList_GET_SIZE(held);
+    bool same = PySequence_Fast_GET_SIZE(seq) == n;
+    for (Py_ssize_t k = 0; same && k < n; ++k) same = PySequence_Fast_GET_ITEM(seq, k) == PyList_GET_ITEM(held, k);
+    Py_DECREF(seq);
+    return PyBool_FromLong(same);
+}
+
 PyMethodDef methods[] = {
     {"collect_step", collect<true>, METH_VARARGS, "table of the parameters that have a gradient"},
     {"collect_params", collect<false>, METH_VARARGS, "table of all parameters"},
     {"collect_grads", collect_grads, METH_VARARGS, "table of the gradients"},
+    {"same_tensors", same_tensors, METH_VARARGS, "whether two sequences hold the same objects"},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -390,19 +390,20 @@ class MultiAdamW(torch.optim.Optimizer):
         if max_norm is not None and not clip >= 0.0:
             raise ValueError(f"MultiAdamW: max_norm={max_norm} must not be negative or NaN")
         _lib.check_device(self.grad_norm)
-        keep, total = [], 0
-        for k, (g, st) in enumerate(zip(self.param_groups, self._groups)):
-            if len(g["params"]) != len(st.params):
+        keep, total, same = [], 0, _lib.host().same_tensors
+        for g, st in zip(self.param_groups, self._groups):
+            if not same(g["params"], st.params):
                 raise RuntimeError("MultiAdamW: a param group's list of tensors was changed")
             self._check_group(g)
             if g["state_bits"] != st.bits:
                 raise RuntimeError(f"MultiAdamW: state_bits of a group was changed from {st.bits} to {g['state_bits']}")
+            if isinstance(g["lr"], torch.Tensor) and g["lr"].device != st.device:
+                raise RuntimeError(f"MultiAdamW: lr lives on {g['lr'].device}, the parameters on {st.device}")
+        for k, (g, st) in enumerate(zip(self.param_groups, self._groups)):
             n, kept = st.collect()
             total += n
             keep.append(kept)
             c, lr = st.c, g["lr"]
-            if isinstance(lr, torch.Tensor) and lr.device != st.device:
-                raise RuntimeError(f"MultiAdamW: lr lives on {lr.device}, the parameters on {st.device}")
             c.lr, c.lr_dev = (0.0, lr.data_ptr()) if isinstance(lr, torch.Tensor) else (float(lr), None)
             (c.beta1, c.beta2), c.eps, c.weight_decay = g["betas"], g["eps"], g["weight_decay"]
             self._c[k] = c

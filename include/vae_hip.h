@@ -577,7 +577,7 @@ int vae_adamw_clip_step_elbo(float* params, const float* grads, float* exp_avg, 
  * fills n elements of it; the rest of its last block is padding that is zero and stays zero.  No two tensors share a block.
  * 8-bit moments: one byte per element and one base per block and moment, bases[2 * block] for exp_avg, bases[2 * block + 1] for
  * exp_avg_sq.  Code c > 0 stands for the fp32 value whose bits are (base + c) << 20, code 0 for zero; exp_avg: c in the low 7
- * bits, sign in bit 7, 0x80 = not finite; exp_avg_sq: 255 = not finite.
+ * bits, sign in bit 7, 0x80 = not finite; exp_avg_sq: 255 = not finite: infinite, or beside 0x80 NaN.
  * bf16 parameters: remainder[] and the parameter make a 32-bit master, |master| bits = (|param| bits << 16) + remainder. */
 #define VAE_MT_MAX_TENSORS 65536
 #define VAE_MT_MAX_GROUPS 64
@@ -623,10 +623,14 @@ int vae_multi_adamw_step(const vae_mt_group* groups, int ngroups, double* partia
 /* out[block * 256 + k] = 32-bit value of parameter element k (master of a bf16 parameter); padding of listed tensors = 0.
  * Gradients are not looked at. */
 int vae_multi_master(const vae_mt_tensor* tensors, int count, const short* remainder, float* out, long nblocks, void* stream);
-/* 8-bit moments -> fp32, or (bf16_out) bf16, which holds their values exactly */
+/* 8-bit moments -> fp32, or (VAE_M8_BF16) bf16, which holds their values exactly.  exp_avg_sq's code 255 reads as NaN; with VAE_M8_INF as
+ * infinity where exp_avg's code is finite, which is what the step takes it for. */
+#define VAE_M8_BF16 1
+#define VAE_M8_INF 256
 int vae_moments8_unpack(const void* exp_avg_q, const void* exp_avg_sq_q, const short* bases, void* exp_avg, void* exp_avg_sq,
-                        long nblocks, int bf16_out, void* stream);
-/* fp32 moments -> 8 bits, rounded to nearest */
+                        long nblocks, int flags, void* stream);
+/* fp32 moments -> 8 bits, rounded to nearest.  An infinite exp_avg_sq makes its exp_avg 0; one that is NaN reads as infinite afterwards
+ * unless exp_avg is not finite either. */
 int vae_moments8_pack(const float* exp_avg, const float* exp_avg_sq, void* exp_avg_q, void* exp_avg_sq_q, short* bases,
                       long nblocks, void* stream);
 

@@ -129,3 +129,65 @@ def test_a_list_that_holds_other_tensors_is_refused(O, change):
     group["params"] = list(ps)
     opt.step()
     assert not torch.equal(ps[0], kept[0])
+
+
+# ------------------------------------------------------------------------------------------------ the end of fp32's range
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("value", [6e20, -1e25, 3e38])
+def test_a_gradient_whose_square_passes_fp32s_range(O, dtype, value):
+    """(1 - beta2) g^2 is infinite from 5.8e20 on: the element's step is 0 from there on, whatever the moments' width, and the decay goes on.
+    decay * p of both widths is one product of the same numbers, so the values are equal bit for bit.  The other elements, those of its block
+    among them, are as if its gradient had been 0."""
+    ps = [torch.nn.Parameter(torch.full((900,), 0.5, dtype=dtype, device=DEV)) for _ in range(3)]
+    full, small, other = (O.MultiAdamW([p], lr=1e-2, weight_decay=0.1, state_bits=b) for p, b in zip(ps, (32, 8, 8)))
+    for t in range(6):
+        g = torch.randn(900, device=DEV, generator=torch.Generator(DEV).manual_seed(t)).to(dtype)
+        for k, p in enumerate(ps):
+            p.grad = g.clone()
+            p.grad[300] = value if k < 2 and t == 1 else 0.0
+        for o in (full, small, other):
+            o.step()
+        assert all(bool(torch.isfinite(p).all()) for p in ps), t
+        if t >= 1:
+            assert torch.equal(full.flat_master()[300], small.flat_master()[300]), t
+        away = torch.ones(900, dtype=torch.bool, device=DEV)
+        away[300] = False
+        assert torch.equal(ps[1][away], ps[2][away]), t
+    assert bool(torch.isinf(full.flat_moments()[1][300]))
+    m, v = small.flat_moments()
+    assert bool(torch.isfinite(m).all()) and bool(torch.isinf(v[300])) and int(torch.isfinite(v[:900]).sum()) == 899
+
+
+def test_an_infinite_second_moment_goes_from_one_width_to_the_other(O):
+    p, q = (torch.nn.Parameter(torch.full((600,), 0.5, device=DEV)) for _ in range(2))
+    a, b = O.MultiAdamW([p], lr=1e-2, state_bits=8), O.MultiAdamW([q], lr=1e-2)
+    for x, o in ((p, a), (q, b)):
+        x.grad = torch.ones(600, device=DEV)
+        x.grad[77], x.grad[300], x.grad[301] = 1e22, float("nan"), float("inf")
+        o.step()
+    for src, bits in ((a, 32), (b, 8)):
+        r = torch.nn.Parameter(torch.full((600,), 0.5, device=DEV))
+        c = O.MultiAdamW([r], lr=1e-2, state_bits=bits)
+        c.load_state_dict(src.state_dict())
+        m, v = c.flat_moments()
+        assert bool(torch.isfinite(m[77])) and bool(torch.isinf(v[77]))
+        r.grad = torch.ones(600, device=DEV)
+        c.step()
+        fine = torch.isfinite(r)
+        assert bool(fine[77]) and not bool(fine[300]) and not bool(fine[301]) and int(fine.sum()) == 598
+        assert float(r.detach()[77]) == float(torch.tensor(0.5) * torch.tensor(1 - 1e-2 * 0.01, dtype=F32))       # the decay alone
+
+
+def test_a_second_moment_that_is_nan_is_not_taken_for_an_infinite_one(O):
+    """a state of another origin: NaN in exp_avg_sq beside a finite exp_avg makes the parameter NaN in both widths, as in torch"""
+    for bits in (32, 8):
+        p = torch.nn.Parameter(torch.full((600,), 0.5, device=DEV))
+        opt = O.MultiAdamW([p], state_bits=bits)
+        m, v = torch.ones(600, device=DEV), torch.ones(600, device=DEV)
+        v[300] = float("nan")
+        opt.load_state_dict({"state": {0: {"step": 3.0, "exp_avg": m, "exp_avg_sq": v}}, "param_groups": [{"params": [0]}]})
+        assert not bool(torch.isnan(m).any())       # what was handed over stays as it was
+        p.grad = torch.ones(600, device=DEV)
+        for _ in range(2):
+            opt.step()
+            assert bool(torch.isnan(p[300])) and int(torch.isnan(p).sum()) == 1

@@ -54,3 +54,9 @@ def test_lists_are_compared_by_identity():
     assert same(tuple(ps), ps)       # any sequence will do
     with pytest.raises(TypeError):
         same(3, ps)
+
+
+def test_moments_unpack_refuses_unknown_flags():
+    for flags in (2, 4, -1, 257 + 2):
+        with pytest.raises(RuntimeError, match="unknown flags"):
+            L.call("vae_moments8_unpack", 4096, 4096, 4096, 4096, 4096, 1, flags, None)

@@ -175,6 +175,7 @@ class MtGroup(ctypes.Structure):
 
 
 MT_PARAM_BF16, MT_GRAD_BF16, MT_BLOCK, MT_MAX_GROUPS, MT_MAX_TENSORS = 1, 2, 256, 64, 65536      # VAE_MT_* of include/vae_hip.h
+M8_BF16, M8_INF = 1, 256                 # VAE_M8_*
 MT_STRIDED = 256                         # STRIDED of csrc/host_collect.cpp
 MT_MIN_EPS8 = 1e-12                      # VAE_MT_MIN_EPS8
 ABI_VERSION = 3                          # VAE_HIP_VERSION of the include/vae_hip.h these signatures were written for

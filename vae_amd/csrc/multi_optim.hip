@@ -12,7 +12,9 @@
 // and three mantissa bits, 8 levels per octave.  Code c > 0 stands for level base + c, code 0 for zero.
 //   exp_avg    : bit 7 = sign, c = 1..127 (15.9 octaves below the block's largest magnitude); 0x80 = not finite
 //   exp_avg_sq : c = 1..254 (31.75 octaves); a positive value always gets c >= 1, because m / (sqrt(0) + eps) of a value
-//                that had only been rounded to zero would be a step of size lr * m / eps; 255 = not finite
+//                that had only been rounded to zero would be a step of size lr * m / eps; 255 = infinite, or beside 0x80 NaN
+// A gradient from 5.8e20 on has a square that makes exp_avg_sq infinite.  Its element then takes no more steps, as with moments in 32 bits;
+// exp_avg has no further use there and is held as 0, so that its block's base does not see it.
 // The base depends on the finite values only, so a NaN in a gradient stays in its own element.
 // Rounding adds d in [0, 2^20) to the bits before the shift.  To nearest (d = 2^19) would not do: with beta2 = 0.999 a step moves
 // exp_avg_sq by at most 0.1 % where its gradient has stopped, a level is 6 to 12 % wide, and it would stay where it is for good.
@@ -385,9 +387,9 @@ __device__ __forceinline__ float unpack_m(uint32_t q, int base) {
     x |= (q & 128u) << 24;
     return __uint_as_float(q == 128u ? 0x7FC00000u : x);
 }
-__device__ __forceinline__ float unpack_v(uint32_t q, int base) {
+__device__ __forceinline__ float unpack_v(uint32_t q, int base, bool inf) {
     const uint32_t x = q ? (uint32_t)(base + (int)q) << 20 : 0u;
-    return __uint_as_float(q == 255u ? 0x7FC00000u : x);
+    return __uint_as_float(q == 255u ? (inf ? 0x7F800000u : 0x7FC00000u) : x);
 }
 // Does one of the four codes of a word mean "not finite"?  (a byte of x is zero: (x - 01..01) & ~x & 80..80 is not)
 __device__ __forceinline__ bool odd_codes(uint32_t qm, uint32_t qv) {
@@ -465,7 +467,7 @@ struct AdamBlock {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 if (((qm >> 8 * k) & 255u) == 128u) m[k] = __uint_as_float(0x7FC00000u);
-                if (((qv >> 8 * k) & 255u) == 255u) v[k] = __uint_as_float(0x7FC00000u);
+                if (((qv >> 8 * k) & 255u) == 255u) v[k] = __uint_as_float(0x7F800000u);      // NaN only beside one in m, which the step gets from there
             }
         }
     }
@@ -484,7 +486,9 @@ struct AdamBlock {
             xm = xv = 0;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const uint32_t x = __float_as_uint(m[k]) & 0x7FFFFFFFu, y = __float_as_uint(v[k]) & 0x7FFFFFFFu;
+                const uint32_t y = __float_as_uint(v[k]) & 0x7FFFFFFFu;
+                if (y == 0x7F800000u && finite_bits(__float_as_uint(m[k]) & 0x7FFFFFFFu)) m[k] = 0.f;
+                const uint32_t x = __float_as_uint(m[k]) & 0x7FFFFFFFu;
                 if (!finite_bits(x)) { odd_m |= 128u << 8 * k; m[k] = 0.f; }
                 else if (x > 0x7F700000u) m[k] = copysignf(__uint_as_float(0x7F700000u), m[k]);
                 if (!finite_bits(y)) { odd_v |= 255u << 8 * k; v[k] = 0.f; }
@@ -666,7 +670,7 @@ __global__ __launch_bounds__(256) void multi_master_kernel(const MtTable tab, co
 // 8 elements a thread: 16-byte stores
 template <bool BF, bool NT>
 __global__ __launch_bounds__(256) void moments8_unpack_kernel(const uint8_t* __restrict__ qm, const uint8_t* __restrict__ qv,
-                                                              const short2* __restrict__ base, void* __restrict__ m, void* __restrict__ v, long n) {
+                                                              const short2* __restrict__ base, void* __restrict__ m, void* __restrict__ v, long n, bool inf) {
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (long)gridDim.x * 2048) {
@@ -675,8 +679,9 @@ __global__ __launch_bounds__(256) void moments8_unpack_kernel(const uint8_t* __r
         float x[8], y[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            x[k] = unpack_m((a[k / 4] >> 8 * (k & 3)) & 255u, b.x);
-            y[k] = unpack_v((c[k / 4] >> 8 * (k & 3)) & 255u, b.y);
+            const uint32_t p = (a[k / 4] >> 8 * (k & 3)) & 255u;
+            x[k] = unpack_m(p, b.x);
+            y[k] = unpack_v((c[k / 4] >> 8 * (k & 3)) & 255u, b.y, inf && p != 128u);
         }
         if (BF) {      // 4 significant bits: exact
             st<NT>((u32x4*)((bf16_t*)m + i), u32x4{pack2bf(x[0], x[1]), pack2bf(x[2], x[3]), pack2bf(x[4], x[5]), pack2bf(x[6], x[7])});
@@ -952,7 +957,9 @@ static int blocks_grid(long nblocks, int per) {
 }
 
 extern "C" int vae_moments8_unpack(const void* exp_avg_q, const void* exp_avg_sq_q, const short* bases, void* exp_avg, void* exp_avg_sq, long nblocks,
-                                   int bf16_out, void* stream) {
+                                   int flags, void* stream) {
+    VAE_CHECK((flags & ~(VAE_M8_BF16 | VAE_M8_INF)) == 0, "vae_moments8_unpack: unknown flags 0x%x", flags);
+    const bool bf16_out = flags & VAE_M8_BF16;
     VAE_CHECK(nblocks >= 0 && nblocks < (1L << 32), "vae_moments8_unpack: nblocks=%ld", nblocks);
     if (nblocks == 0) return 0;
     VAE_CHECK(exp_avg_q && exp_avg_sq_q && bases && exp_avg && exp_avg_sq, "vae_moments8_unpack: null pointer");
@@ -964,7 +971,7 @@ extern "C" int vae_moments8_unpack(const void* exp_avg_q, const void* exp_avg_sq
         const auto kernel = bf16_out ? (nt ? moments8_unpack_kernel<true, true> : moments8_unpack_kernel<true, false>)
                                      : (nt ? moments8_unpack_kernel<false, true> : moments8_unpack_kernel<false, false>);
         hipLaunchKernelGGL(kernel, dim3(blocks_grid(nblocks, 8)), dim3(256), 0, (hipStream_t)stream, (const uint8_t*)exp_avg_q,
-                           (const uint8_t*)exp_avg_sq_q, (const short2*)bases, exp_avg, exp_avg_sq, nblocks * MT_BLOCK);
+                           (const uint8_t*)exp_avg_sq_q, (const short2*)bases, exp_avg, exp_avg_sq, nblocks * MT_BLOCK, (flags & VAE_M8_INF) != 0);
     }
     VAE_LAUNCH_CHECK("moments8_unpack_kernel");
     return 0;

@@ -437,7 +437,7 @@ class MultiAdamW(torch.optim.Optimizer):
     @staticmethod
     def _unpack(st, qm, qv, bases, m, v):
         _lib.call("vae_moments8_unpack", qm.data_ptr(), qv.data_ptr(), bases.data_ptr(), m.data_ptr(), v.data_ptr(), bases.shape[0],
-                  int(m.dtype is torch.bfloat16), _lib.current_stream())
+                  _lib.M8_INF | (_lib.M8_BF16 if m.dtype is torch.bfloat16 else 0), _lib.current_stream())
 
     def flat_master(self, group=0):
         """32-bit values of a group's parameters in the state's layout: a bf16 parameter's master, an fp32 parameter itself"""
@@ -573,6 +573,7 @@ class MultiAdamW(torch.optim.Optimizer):
             if full:
                 f32 = scratch(torch.float32)
                 fill(f32, st.view, full, ("exp_avg", "exp_avg_sq"))
+                f32[0].masked_fill_(f32[1].isnan(), float("nan"))       # alone in exp_avg_sq it would be taken for infinity
                 _lib.call("vae_moments8_pack", f32[0].data_ptr(), f32[1].data_ptr(), q[0].data_ptr(), q[1].data_ptr(), bases.data_ptr(),
                           bases.shape[0], _lib.current_stream())
             else:

@@ -191,3 +191,23 @@ def test_a_second_moment_that_is_nan_is_not_taken_for_an_infinite_one(O):
         for _ in range(2):
             opt.step()
             assert bool(torch.isnan(p[300])) and int(torch.isnan(p).sum()) == 1
+
+
+# ------------------------------------------------------------------------------------------------ state_dicts
+@pytest.mark.parametrize("key, other, limit", [("exp_avg_base", "exp_avg_sq_base", 0x7F7 - 127), ("exp_avg_sq_base", "exp_avg_base", 0x7F7 - 254)])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_bases_end_where_their_largest_code_is_fp32s_last_level(O, key, other, limit, bits):
+    n = [700, 300]
+    _, src = stepped(O, n, F32, 8)
+    sd = copy.deepcopy(src.state_dict())
+    _, dst = stepped(O, n, F32, bits, seed=1)
+    was = everything(dst)
+    for bad in (limit + 1, 0x7F7, -1):
+        sd["state"][1][key] = torch.tensor([limit, bad], dtype=torch.int32, device=DEV)
+        with pytest.raises(ValueError, match="no levels of finite numbers"):
+            dst.load_state_dict(sd)
+        assert same(everything(dst), was)
+    sd["state"][1][key] = torch.tensor([limit, 0], dtype=torch.int32, device=DEV)
+    dst.load_state_dict(sd)
+    m, v = dst.flat_moments()
+    assert bool(torch.isfinite(m).all()) and bool(torch.isfinite(v).all()) and bool((v >= 0).all())

@@ -499,11 +499,12 @@ class MultiAdamW(torch.optim.Optimizer):
                     for key, x in state.get(i, {}).items()} for i in saved["params"]]
             for k, e in enumerate(row):
                 self._check_entry(st, k, e)
-            bases = [e[key].reshape(-1) for e in row if "exp_avg_q" in e for key in ("exp_avg_base", "exp_avg_sq_base")]
-            if bases:
-                low, high = torch.cat(bases).aminmax() if sum(b.numel() for b in bases) else (0, 0)
-                if int(low) < 0 or int(high) > 0x7F7:
-                    raise ValueError(f"MultiAdamW: bases from {int(low)} to {int(high)} are no levels of finite numbers")
+            for key, limit in (("exp_avg_base", 0x7F7 - 127), ("exp_avg_sq_base", 0x7F7 - 254)):       # + the largest code: fp32's last level
+                bases = [e[key].reshape(-1) for e in row if "exp_avg_q" in e]
+                if sum(b.numel() for b in bases):
+                    low, high = torch.stack(torch.cat(bases).aminmax()).tolist()
+                    if low < 0 or high > limit:
+                        raise ValueError(f"MultiAdamW: {key} from {low} to {high}: above {limit} they are no levels of finite numbers")
             entries.append(row)
         merged = []
         for saved, g in zip(groups, self.param_groups):

@@ -211,3 +211,19 @@ def test_bases_end_where_their_largest_code_is_fp32s_last_level(O, key, other, l
     dst.load_state_dict(sd)
     m, v = dst.flat_moments()
     assert bool(torch.isfinite(m).all()) and bool(torch.isfinite(v).all()) and bool((v >= 0).all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_dict_taken_before_a_step_fits_together_after_it(O, bits):
+    """codes and bases are views of the same live state: an old dict gives the present moments, not new codes with old bases"""
+    n = [700, 300]
+    ps, opt = stepped(O, n, F32, bits)
+    sd = opt.state_dict()
+    for t in range(3):       # moments of another magnitude, hence of other bases
+        for p, g in zip(ps, tensors(n, F32, 0, 80 + t, 1e4)[0]):
+            p.grad = g
+        opt.step()
+    m, v = opt.flat_moments()
+    m, v = m.clone(), v.clone()
+    opt.load_state_dict(sd)
+    assert same(opt.flat_moments(), (m, v))

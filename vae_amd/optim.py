@@ -463,19 +463,18 @@ class MultiAdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def state_dict(self):
         """torch's layout: ``state[i]`` of the i-th parameter with ``step``, ``exp_avg``, ``exp_avg_sq`` in the parameter's shape (views
-        of the live state, as in torch).  8-bit moments: the codes ``exp_avg_q``, ``exp_avg_sq_q`` in the order of the
-        parameter's memory and the blocks' ``exp_avg_base``, ``exp_avg_sq_base``.  bf16 parameters: ``remainder`` too."""
+        of the live state, as in torch; ``step`` is a copy).  8-bit moments: the codes ``exp_avg_q``, ``exp_avg_sq_q`` in the order of the
+        parameter's memory and the blocks' ``exp_avg_base``, ``exp_avg_sq_base`` (int16).  bf16 parameters: ``remainder`` too."""
         state, groups, at = {}, [], 0
         for g, st in zip(self.param_groups, self._groups):
             steps = st.steps.tolist()
-            bases = st.bases.t().contiguous().int() if st.bits == 8 else None
             for k in range(len(st.params)):
                 e = {"step": torch.tensor(float(steps[k]), dtype=torch.float32 if steps[k] < 1 << 24 else torch.float64)}
                 if st.bits == 32:
                     e["exp_avg"], e["exp_avg_sq"] = st.view(st.exp_avg, k), st.view(st.exp_avg_sq, k)
                 else:
                     e["exp_avg_q"], e["exp_avg_sq_q"] = st.run(st.exp_avg, k), st.run(st.exp_avg_sq, k)
-                    e["exp_avg_base"], e["exp_avg_sq_base"] = (bases[j, st.rows(k)] for j in (0, 1))
+                    e["exp_avg_base"], e["exp_avg_sq_base"] = (st.bases[st.rows(k), j] for j in (0, 1))
                     e["stride"] = st.strides[k]
                 if st.dtypes[k] is torch.bfloat16:
                     e["remainder"] = st.view(st.remainder, k)

@@ -227,3 +227,35 @@ def test_a_state_dict_taken_before_a_step_fits_together_after_it(O, bits):
     m, v = m.clone(), v.clone()
     opt.load_state_dict(sd)
     assert same(opt.flat_moments(), (m, v))
+
+
+def test_other_keys_of_the_groups_are_loaded(O):
+    """what a cyclic scheduler and the user keep in a group comes back: the schedule goes on where it was"""
+    def make():
+        ps = [torch.nn.Parameter(torch.ones(300, device=DEV)) for _ in range(2)]
+        return O.MultiAdamW([{"params": ps[:1], "name": "first"}, {"params": ps[1:], "name": "second", "state_bits": 8}], lr=1e-3)
+    sched = lambda o, last=-1: torch.optim.lr_scheduler.OneCycleLR(o, max_lr=[0.1, 0.2], total_steps=20, last_epoch=last)  # noqa: E731
+    a = make()
+    s = sched(a)
+    for _ in range(5):
+        a.step(), s.step()
+    saved = copy.deepcopy(a.state_dict())
+    saved["param_groups"][0]["tags"] = ["x"]
+    b = make()
+    b.param_groups[0]["name"] = b.param_groups[1]["name"] = "?"
+    b.param_groups[0]["own"] = 7
+    b.load_state_dict(saved)
+    assert [g["name"] for g in b.param_groups] == ["first", "second"] and [g["state_bits"] for g in b.param_groups] == [32, 8]
+    assert b.param_groups[0]["tags"] == ["x"] and b.param_groups[0]["tags"] is not saved["param_groups"][0]["tags"] and b.param_groups[0]["own"] == 7
+    r = sched(b, s.last_epoch)
+    s.step()
+    for _ in range(5):
+        assert [(g["lr"], g["betas"], g["max_lr"], g["min_lr"]) for g in a.param_groups] == [(g["lr"], g["betas"], g["max_lr"], g["min_lr"]) for g in b.param_groups]
+        a.step(), b.step(), s.step(), r.step()
+    # torch's switches are not this optimizer's, and its moments' width stays
+    q = torch.nn.Parameter(torch.ones(300, device=DEV))
+    c = O.MultiAdamW([q], state_bits=8)
+    c.load_state_dict(torch.optim.AdamW([torch.nn.Parameter(torch.ones(300, device=DEV))], lr=0.5, fused=True).state_dict())
+    g = c.param_groups[0]
+    assert g["lr"] == 0.5 and g["state_bits"] == 8 and not {"fused", "foreach", "amsgrad", "maximize", "capturable", "differentiable"} & set(g)
+    assert g["params"][0] is q

@@ -6,6 +6,7 @@ Same update rule and defaults as the reference's optimizer
 eps 1e-8, weight_decay 0.01) preceded by clip_grad_norm_(max_norm) (train.py:336)."""
 from __future__ import annotations
 
+import copy
 import ctypes
 import threading
 
@@ -274,6 +275,10 @@ class _GroupState:
         return slice(self.start[k], self.start[k] + -(-self.n[k] // _lib.MT_BLOCK))
 
 
+# keys of a saved param group that stay as they are here: the tensors, the moments' width, and torch's choices among its own forms
+_NOT_LOADED = {"params", "state_bits", "amsgrad", "maximize", "foreach", "fused", "capturable", "differentiable", "decoupled_weight_decay"}
+
+
 class MultiAdamW(torch.optim.Optimizer):
     """AdamW over any number of separate fp32 or bf16 tensors, with the gradient clip of the loop in the same pass.
 
@@ -486,7 +491,8 @@ class MultiAdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict):
         """Takes what ``state_dict`` gives, of this class or of torch.optim.AdamW, and converts between moments in 32 and in 8 bits
-        (to nearest) where the two differ.  A parameter without an entry starts from zero.  Nothing is written if an entry does not fit."""
+        (to nearest) where the two differ.  A parameter without an entry starts from zero.  The groups' other keys (a scheduler's, the user's)
+        are taken over too, the moments' width is not.  Nothing is written if an entry does not fit."""
         groups, state = state_dict["param_groups"], state_dict["state"]
         if [len(g["params"]) for g in groups] != [len(st.params) for st in self._groups]:
             raise ValueError("MultiAdamW: the state_dict's param groups have other lengths")
@@ -509,7 +515,7 @@ class MultiAdamW(torch.optim.Optimizer):
         for saved, g in zip(groups, self.param_groups):
             if saved.get("amsgrad") or saved.get("maximize"):
                 raise ValueError("MultiAdamW: the state_dict is of an AdamW with amsgrad or maximize, which is another rule")
-            new = {key: x for key, x in saved.items() if key in ("lr", "betas", "eps", "weight_decay", "initial_lr")}
+            new = {key: copy.deepcopy(x) for key, x in saved.items() if key not in _NOT_LOADED}
             if "lr" in new:
                 new["lr"] = float(new["lr"])
             if "betas" in new:
@@ -518,7 +524,7 @@ class MultiAdamW(torch.optim.Optimizer):
             merged.append(new)
         for new, g, st, row in zip(merged, self.param_groups, self._groups, entries):
             for key, x in new.items():
-                if isinstance(g.get(key), torch.Tensor):
+                if key in ("lr", "initial_lr") and isinstance(g.get(key), torch.Tensor):
                     g[key].fill_(x)       # a captured step reads this tensor
                 else:
                     g[key] = x

@@ -259,3 +259,31 @@ def test_other_keys_of_the_groups_are_loaded(O):
     g = c.param_groups[0]
     assert g["lr"] == 0.5 and g["state_bits"] == 8 and not {"fused", "foreach", "amsgrad", "maximize", "capturable", "differentiable"} & set(g)
     assert g["params"][0] is q
+
+
+def test_hooks_of_the_state_dict(O):
+    n, seen = [300], []
+    _, opt = stepped(O, n, F32, 32)
+    h = [opt.register_state_dict_pre_hook(lambda o: seen.append(("pre", o is opt))),
+         opt.register_state_dict_post_hook(lambda o, sd: {**sd, "extra": 5}),
+         opt.register_load_state_dict_pre_hook(lambda o, sd: seen.append(("load", o is opt, sd["extra"]))),
+         opt.register_load_state_dict_pre_hook(lambda o, sd: {**sd, "param_groups": [{**sd["param_groups"][0], "lr": 0.25}]}),
+         opt.register_load_state_dict_post_hook(lambda o: seen.append(("loaded", o is opt, o.param_groups[0]["lr"])))]
+    sd = opt.state_dict()
+    assert sd["extra"] == 5 and seen == [("pre", True)]
+    was = everything(opt)
+    opt.load_state_dict(sd)
+    assert seen[1:] == [("load", True, 5), ("loaded", True, 0.25)] and sd["param_groups"][0]["lr"] == 1e-3 and same(everything(opt), was)
+    for x in h:
+        x.remove()
+    opt.load_state_dict(sd)
+    assert len(seen) == 3 and "extra" not in opt.state_dict() and opt.param_groups[0]["lr"] == 1e-3
+
+
+def test_a_hook_that_changes_the_state_dict_changes_a_copy(O):
+    _, opt = stepped(O, [300], F32, 8)
+    sd = opt.state_dict()
+    h = opt.register_load_state_dict_pre_hook(lambda o, d: d.update(state={}))       # nothing returned: the dict it was given counts
+    opt.load_state_dict(sd)
+    h.remove()
+    assert len(sd["state"]) == 1 and not bool(opt.flat_moments()[0].any())

@@ -470,6 +470,8 @@ class MultiAdamW(torch.optim.Optimizer):
         """torch's layout: ``state[i]`` of the i-th parameter with ``step``, ``exp_avg``, ``exp_avg_sq`` in the parameter's shape (views
         of the live state, as in torch; ``step`` is a copy).  8-bit moments: the codes ``exp_avg_q``, ``exp_avg_sq_q`` in the order of the
         parameter's memory and the blocks' ``exp_avg_base``, ``exp_avg_sq_base`` (int16).  bf16 parameters: ``remainder`` too."""
+        for hook in self._optimizer_state_dict_pre_hooks.values():
+            hook(self)
         state, groups, at = {}, [], 0
         for g, st in zip(self.param_groups, self._groups):
             steps = st.steps.tolist()
@@ -486,13 +488,21 @@ class MultiAdamW(torch.optim.Optimizer):
                 state[at + k] = e
             groups.append({**{key: x for key, x in g.items() if key != "params"}, "params": list(range(at, at + len(st.params)))})
             at += len(st.params)
-        return {"state": state, "param_groups": groups}
+        state_dict = {"state": state, "param_groups": groups}
+        for hook in self._optimizer_state_dict_post_hooks.values():
+            new = hook(self, state_dict)
+            state_dict = state_dict if new is None else new
+        return state_dict
 
     @torch.no_grad()
     def load_state_dict(self, state_dict):
         """Takes what ``state_dict`` gives, of this class or of torch.optim.AdamW, and converts between moments in 32 and in 8 bits
         (to nearest) where the two differ.  A parameter without an entry starts from zero.  The groups' other keys (a scheduler's, the user's)
         are taken over too, the moments' width is not.  Nothing is written if an entry does not fit."""
+        state_dict = dict(state_dict)       # a hook may exchange its parts
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            new = hook(self, state_dict)
+            state_dict = state_dict if new is None else new
         groups, state = state_dict["param_groups"], state_dict["state"]
         if [len(g["params"]) for g in groups] != [len(st.params) for st in self._groups]:
             raise ValueError("MultiAdamW: the state_dict's param groups have other lengths")
@@ -535,6 +545,8 @@ class MultiAdamW(torch.optim.Optimizer):
                 if have:
                     torch._foreach_copy_([st.view(st.remainder, k) for k in have], [row[k]["remainder"].view(st.shapes[k]) for k in have])
             self._load_moments(st, row)
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
 
     @staticmethod
     def _check_entry(st, k, e):

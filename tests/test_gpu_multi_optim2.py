@@ -287,3 +287,29 @@ def test_a_hook_that_changes_the_state_dict_changes_a_copy(O):
     opt.load_state_dict(sd)
     h.remove()
     assert len(sd["state"]) == 1 and not bool(opt.flat_moments()[0].any())
+
+
+def test_entries_of_another_form_change_nothing(O):
+    """codes in two dims, a remainder that is no view of the parameter's shape, a remainder of another type: refused before the first write, or
+    taken for what they are"""
+    n = [700, 64]
+    ps, opt = stepped(O, n, BF16, 8)
+    was, lr = everything(opt), opt.param_groups[0]["lr"]
+    own = copy.deepcopy(opt.state_dict())
+
+    def change(key, value):
+        sd = copy.deepcopy(own)
+        sd["param_groups"][0]["lr"] = 7.0
+        sd["state"][1][key] = value
+        return sd
+    e = own["state"][1]
+    for key, value, error in (("remainder", e["remainder"].float(), TypeError), ("exp_avg_base", e["exp_avg_base"].float(), TypeError),
+                              ("exp_avg_sq_q", e["exp_avg_sq_q"].int(), TypeError), ("remainder", e["remainder"][:63], ValueError)):
+        with pytest.raises(error, match=key if "_q" not in key else "codes"):
+            opt.load_state_dict(change(key, value))
+        assert same(everything(opt), was) and opt.param_groups[0]["lr"] == lr
+    for key in ("remainder", "exp_avg_q", "exp_avg_sq_q"):       # the same elements in the same order, in another shape
+        wide = torch.stack([e[key].view(8, 8)] * 2, 2)[:, :, 0]
+        assert not wide.is_contiguous()
+        opt.load_state_dict(change(key, wide))
+        assert same(everything(opt), was) and opt.param_groups[0]["lr"] == 7.0

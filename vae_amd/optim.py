@@ -543,7 +543,9 @@ class MultiAdamW(torch.optim.Optimizer):
                 st.remainder.zero_()
                 have = [k for k, e in enumerate(row) if "remainder" in e and st.dtypes[k] is torch.bfloat16]
                 if have:
-                    torch._foreach_copy_([st.view(st.remainder, k) for k in have], [row[k]["remainder"].view(st.shapes[k]) for k in have])
+                    src = [row[k]["remainder"] for k in have]
+                    torch._foreach_copy_([st.view(st.remainder, k) for k in have],
+                                         [x if tuple(x.shape) == st.shapes[k] else x.reshape(st.shapes[k]) for k, x in zip(have, src)])
             self._load_moments(st, row)
         for hook in self._optimizer_load_state_dict_post_hooks.values():
             hook(self)
@@ -561,6 +563,8 @@ class MultiAdamW(torch.optim.Optimizer):
         for key in e:
             if key in ("exp_avg", "exp_avg_sq", "exp_avg_q", "exp_avg_sq_q", "remainder"):
                 fits(key, st.n[k])
+        if "remainder" in e and st.dtypes[k] is torch.bfloat16 and e["remainder"].dtype is not torch.int16:
+            raise TypeError(f"MultiAdamW: the remainder of parameter {k} is {e['remainder'].dtype}, not int16")
         if "exp_avg_q" in e:
             for key in ("exp_avg_sq_q", "exp_avg_base", "exp_avg_sq_base"):
                 if key not in e:
@@ -568,6 +572,8 @@ class MultiAdamW(torch.optim.Optimizer):
             rows = st.rows(k)
             for key in ("exp_avg_base", "exp_avg_sq_base"):
                 fits(key, rows.stop - rows.start)
+                if e[key].dtype.is_floating_point:
+                    raise TypeError(f"MultiAdamW: {key} of parameter {k} is {e[key].dtype}, not of whole numbers")
             if e["exp_avg_q"].dtype is not torch.uint8 or e["exp_avg_sq_q"].dtype is not torch.uint8:
                 raise TypeError(f"MultiAdamW: the codes of parameter {k} are not uint8")
             if "stride" in e and tuple(e["stride"]) != tuple(st.strides[k]) and st.n[k] > 1:
@@ -585,7 +591,8 @@ class MultiAdamW(torch.optim.Optimizer):
         def fill(dst, view, which, keys):
             if which:
                 for buf, key in zip(dst, keys):
-                    torch._foreach_copy_([view(buf, k) for k in which], [row[k][key] for k in which])
+                    to, src = [view(buf, k) for k in which], [row[k][key] for k in which]
+                    torch._foreach_copy_(to, [x if x.shape == t.shape else x.reshape(t.shape) for x, t in zip(src, to)])
         if st.bits == 8:
             q, bases = (st.exp_avg, st.exp_avg_sq), st.bases
             if full:

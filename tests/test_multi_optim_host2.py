@@ -60,3 +60,19 @@ def test_moments_unpack_refuses_unknown_flags():
     for flags in (2, 4, -1, 257 + 2):
         with pytest.raises(RuntimeError, match="unknown flags"):
             L.call("vae_moments8_unpack", 4096, 4096, 4096, 4096, 4096, 1, flags, None)
+
+
+def test_strides_of_dims_of_one_element_do_not_matter(monkeypatch):
+    """a 1x1 convolution in channels_last and contiguous: the same order of elements, other strides"""
+    x = torch.randn(8, 6, 1, 1)
+    a, b = x.to(memory_format=torch.channels_last), x.clone()
+    assert a.stride() != b.stride()
+    st = held(monkeypatch, [torch.nn.Parameter(a)], 8)
+    codes, bases = torch.zeros(48, dtype=torch.uint8), torch.zeros(1, dtype=torch.int16)
+    e = {"step": 1, "exp_avg_q": codes, "exp_avg_sq_q": codes, "exp_avg_base": bases, "exp_avg_sq_base": bases, "stride": b.stride()}
+    optim.MultiAdamW._check_entry(st, 0, e)
+    other = held(monkeypatch, [torch.nn.Parameter(torch.randn(6, 8).t())], 8)
+    for stride in ((6, 1), (1, 6), (8, 1)):
+        with pytest.raises(ValueError, match="order of strides"):
+            optim.MultiAdamW._check_entry(other, 0, {**e, "stride": stride})
+    optim.MultiAdamW._check_entry(other, 0, {**e, "stride": (1, 8)})

@@ -576,7 +576,8 @@ class MultiAdamW(torch.optim.Optimizer):
                     raise TypeError(f"MultiAdamW: {key} of parameter {k} is {e[key].dtype}, not of whole numbers")
             if e["exp_avg_q"].dtype is not torch.uint8 or e["exp_avg_sq_q"].dtype is not torch.uint8:
                 raise TypeError(f"MultiAdamW: the codes of parameter {k} are not uint8")
-            if "stride" in e and tuple(e["stride"]) != tuple(st.strides[k]) and st.n[k] > 1:
+            if "stride" in e and st.n[k] > 1 and (len(e["stride"]) != len(st.shapes[k]) or any(
+                    a != b and size != 1 for a, b, size in zip(e["stride"], st.strides[k], st.shapes[k]))):
                 raise ValueError(f"MultiAdamW: the codes of parameter {k} are in the order of strides {tuple(e['stride'])}, the parameter has {st.strides[k]}")
         elif "exp_avg" in e:
             for key in ("exp_avg", "exp_avg_sq"):

@@ -313,3 +313,36 @@ def test_entries_of_another_form_change_nothing(O):
         assert not wide.is_contiguous()
         opt.load_state_dict(change(key, wide))
         assert same(everything(opt), was) and opt.param_groups[0]["lr"] == 7.0
+
+
+# ------------------------------------------------------------------------------------------------ the loop
+def test_a_model_with_frozen_parameters_is_clipped_in_the_step(O):
+    """the optimizer holds the trainable parameters only: its norm is that of all gradients there are, so it clips while it steps and leaves the
+    gradients alone; where the model has a gradient that the optimizer does not step, the clip runs over the model as before"""
+    from vae_amd.train import _clip_and_step
+    torch.manual_seed(5)
+    net = torch.nn.Sequential(torch.nn.Linear(20, 30), torch.nn.Linear(30, 10)).to(DEV)
+    net[0].requires_grad_(False)
+    opt = O.MultiAdamW([p for p in net.parameters() if p.requires_grad], lr=1e-2)
+    x = torch.randn(8, 20, device=DEV)
+
+    def gradients():
+        opt.zero_grad()
+        for p in net[0].parameters():
+            p.grad = None
+        (net(x) * 50).square().sum().backward()
+        return [p.grad.clone() for p in net[1].parameters()]
+    kept = gradients()
+    norm = R.norm([np64(g) for g in kept])
+    assert norm > 10 and opt.holds(net[1].parameters()) and not opt.holds(net.parameters())
+    _clip_and_step(net, opt, 1.0)
+    assert abs(float(opt.grad_norm) - norm) <= 1.01 * R.EPS24 * norm
+    assert all(torch.equal(p.grad, g) for p, g in zip(net[1].parameters(), kept))
+    net[0].requires_grad_(True)       # now the model has gradients that are not stepped
+    kept, opt.grad_norm = gradients(), torch.full((1,), -1.0, device=DEV)
+    norm = R.norm([np64(p.grad) for p in net.parameters()])
+    frozen = [p.detach().clone() for p in net[0].parameters()]
+    _clip_and_step(net, opt, 1.0)
+    for p, g in zip(net[1].parameters(), kept):       # torch's norm and coefficient in fp32: a sum of 970 squares, off by less than 1e-5
+        within(p.grad, np64(g) / norm, 2e-5 * np.abs(np64(g) / norm))
+    assert same([p.detach() for p in net[0].parameters()], frozen) and float(opt.grad_norm) == -1.0

@@ -367,6 +367,10 @@ class MultiAdamW(torch.optim.Optimizer):
         """whether these are exactly the tensors it steps"""
         return {id(p) for p in parameters} == {id(p) for st in self._groups for p in st.params}
 
+    def holds_gradients(self, parameters):
+        """whether those of these parameters that have a gradient are exactly those that a step takes now (frozen ones do not matter)"""
+        return {id(p) for p in parameters if p.grad is not None} == {id(p) for st in self._groups for p in st.params if p.grad is not None}
+
     def __getstate__(self):
         raise TypeError("MultiAdamW holds device buffers and is not copied or pickled: save state_dict() and load it into a new one")
 

@@ -168,8 +168,8 @@ def train_step(model, optimizer, inputs, config, eps=None, keep_masks=None, max_
 
 def _clip_and_step(model, optimizer, max_norm):
     """clip_grad_norm_(max_norm); optimizer.step() (train.py:336-338).  MultiAdamW clips while it steps, provided that it steps all
-    of the model's parameters: the norm runs over those it holds."""
-    if isinstance(optimizer, MultiAdamW) and optimizer.holds(model.parameters()):
+    of the model's parameters that have a gradient, and no others: the norm runs over those it holds."""
+    if isinstance(optimizer, MultiAdamW) and optimizer.holds_gradients(model.parameters()):
         optimizer.step(max_norm=max_norm)
     else:
         torch.nn.utils.clip_grad_norm_(model.parameters(), max_norm=max_norm)

@@ -346,3 +346,26 @@ def test_a_model_with_frozen_parameters_is_clipped_in_the_step(O):
     for p, g in zip(net[1].parameters(), kept):       # torch's norm and coefficient in fp32: a sum of 970 squares, off by less than 1e-5
         within(p.grad, np64(g) / norm, 2e-5 * np.abs(np64(g) / norm))
     assert same([p.detach() for p in net[0].parameters()], frozen) and float(opt.grad_norm) == -1.0
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_an_infinite_bf16_parameter_written_from_outside_stays_infinite(O, bits):
+    """beside a remainder of either sign: bf16's infinity and a positive remainder would be the bits of a NaN"""
+    n = [2048, 9]
+    ps, opt = stepped(O, n, BF16, bits)
+    r = opt._groups[0].remainder[:2048]
+    assert int((r > 0).sum()) > 100 and int((r < 0).sum()) > 100
+    with torch.no_grad():
+        ps[0][::2], ps[0][1::4], ps[0][3::4] = float("inf"), -float("inf"), float("nan")
+    want = ps[0].detach().float()
+    w = opt.flat_master()[:2048]
+    # a negative remainder makes it the 32-bit number that is rounded to infinity: more than bf16's largest
+    assert bool(torch.isnan(w[3::4]).all()) and not bool(torch.isnan(w[::2]).any()) and not bool(torch.isnan(w[1::4]).any())
+    fine = ~torch.isnan(want)
+    assert torch.equal(w[fine].sign(), want[fine].sign()) and bool((w[fine].abs() > torch.finfo(BF16).max).all())
+    ps[0].grad, ps[1].grad = torch.zeros(2048, dtype=BF16, device=DEV), torch.zeros(9, dtype=BF16, device=DEV)
+    for _ in range(2):
+        ps[0].grad.zero_()
+        opt.step()
+    assert not bool(torch.isnan(ps[0][fine]).any()) and bool(torch.isnan(ps[0][3::4]).all()) and bool(torch.isfinite(ps[1]).all())
+    assert torch.equal(ps[0][fine].float().sign(), want[fine].sign())

@@ -398,10 +398,12 @@ __device__ __forceinline__ bool odd_codes(uint32_t qm, uint32_t qv) {
 }
 
 // ---------------------------------------------------------------- AdamW
-// (parameter, remainder) -> master.  A magnitude below zero can only come of a parameter that was written since, and is 0.
+// (parameter, remainder) -> master.  A magnitude below zero can only come of a parameter that was written since, and is 0; so can an
+// infinity with a positive remainder, which stays infinite (a master that is rounded to one lies below it).  max(t, inf) lets NaN through.
 __device__ __forceinline__ float join_master(bf16_t p, short r) {
-    const uint32_t t = (uint32_t)p << 16;
-    const uint32_t x = (uint32_t)max((int)(t & 0x7FFF0000u) + (int)r, 0);
+    const uint32_t t = (uint32_t)p << 16, mag = t & 0x7FFF0000u;
+    uint32_t x;
+    asm("v_med3_i32 %0, %1, 0, %2" : "=v"(x) : "v"((int)mag + (int)r), "v"(max(mag, 0x7F800000u)));
     return __uint_as_float(x | (t & 0x80000000u));
 }
 // master -> (parameter, remainder): adding half a last place rounds the magnitude, and what the upper half is then too

@@ -76,3 +76,15 @@ def test_strides_of_dims_of_one_element_do_not_matter(monkeypatch):
         with pytest.raises(ValueError, match="order of strides"):
             optim.MultiAdamW._check_entry(other, 0, {**e, "stride": stride})
     optim.MultiAdamW._check_entry(other, 0, {**e, "stride": (1, 8)})
+
+
+# ------------------------------------------------------------------------------------------------ the build
+def test_the_library_builds_where_torch_is_not_installed(tmp_path):
+    """_host.so needs torch's headers; without them make says so and goes on, as libvae_hip.so needs none"""
+    import os
+    import subprocess
+    src = os.path.join(os.path.dirname(L.__file__), "csrc")
+    out = tmp_path / "_host.so"
+    run = lambda python: subprocess.run(["make", "-C", src, f"PYTHON={python}", f"HOST_OUT={out}", str(out)], capture_output=True, text=True)  # noqa: E731
+    r = run("false")
+    assert r.returncode == 0 and not out.exists() and "torch" in r.stdout, r.stdout + r.stderr

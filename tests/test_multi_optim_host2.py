@@ -88,3 +88,16 @@ def test_the_library_builds_where_torch_is_not_installed(tmp_path):
     run = lambda python: subprocess.run(["make", "-C", src, f"PYTHON={python}", f"HOST_OUT={out}", str(out)], capture_output=True, text=True)  # noqa: E731
     r = run("false")
     assert r.returncode == 0 and not out.exists() and "torch" in r.stdout, r.stdout + r.stderr
+
+
+def test_the_walk_takes_the_address_that_may_be_written():
+    """a lazily cloned tensor shares its memory until one of the two is written: what a launch will write has to be its own by then"""
+    a, b = torch.ones(64), torch.ones(64)
+    p = torch.nn.Parameter(torch._lazy_clone(a))
+    p.grad = torch._lazy_clone(b)
+    shared = torch._C._data_address(a), torch._C._data_address(b)
+    jobs = np.zeros(1, optim._JOB)
+    assert L.host().collect_step([p], jobs, np.array([[64, 0, 0, 0]], np.int64), -1) == 1
+    assert jobs["param"][0] != shared[0] and jobs["grad"][0] == shared[1]       # the gradient is only read
+    assert L.host().collect_grads([p], jobs, -1, False) == 1 and jobs["grad"][0] == shared[1]
+    assert L.host().collect_grads([p], jobs, -1, True) == 1 and jobs["grad"][0] != shared[1]

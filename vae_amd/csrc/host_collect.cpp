@@ -67,7 +67,8 @@ PyObject* collect(PyObject*, PyObject* args) {
             if (pk < 0 || gk < 0 || pk != (int)(row[3] & VAE_MT_PARAM_BF16) || (row[3] & STRIDED) || p.numel() != row[0] ||
                 g.numel() != row[0] || !p.is_contiguous() || !g.is_contiguous() || (STEP && (p.is_inference() || p.sizes() != g.sizes())))
                 return PyLong_FromLong(-1);
-            job[live] = {const_cast<void*>(p.const_data_ptr()), g.const_data_ptr(), row[0], (unsigned)row[1], (unsigned)row[2],
+            // mutable: a lazily cloned tensor gets memory of its own
+            job[live] = {STEP ? p.mutable_data_ptr() : const_cast<void*>(p.const_data_ptr()), g.const_data_ptr(), row[0], (unsigned)row[1], (unsigned)row[2],
                          (pk ? VAE_MT_PARAM_BF16 : 0u) | (gk ? VAE_MT_GRAD_BF16 : 0u), 0u};
             ++live;
             if (STEP) written.push_back(&p);
@@ -106,7 +107,7 @@ PyObject* collect_grads(PyObject*, PyObject* args) {
             if (!g.defined()) continue;
             const int gk = kind(g, device);
             if (gk < 0 || !g.is_contiguous() || g.is_inference()) return PyLong_FromLong(-1);
-            const char* a = (const char*)g.const_data_ptr();
+            const char* a = write ? (const char*)g.mutable_data_ptr() : (const char*)g.const_data_ptr();
             job[grads.size()] = {nullptr, a, g.numel(), 0u, 0u, gk ? VAE_MT_GRAD_BF16 : 0u, 0u};
             grads.push_back(&g);
             if (write && g.numel()) spans.emplace_back(a, a + g.nbytes());

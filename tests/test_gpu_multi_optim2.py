@@ -369,3 +369,79 @@ def test_an_infinite_bf16_parameter_written_from_outside_stays_infinite(O, bits)
         opt.step()
     assert not bool(torch.isnan(ps[0][fine]).any()) and bool(torch.isnan(ps[0][3::4]).all()) and bool(torch.isfinite(ps[1]).all())
     assert torch.equal(ps[0][fine].float().sign(), want[fine].sign())
+
+
+# ------------------------------------------------------------------------------------------------ mixed types
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("clip", [False, True])
+def test_a_group_of_all_pairs_of_types(O, bits, clip, shift):
+    """fp32 and bf16 parameters in turn, with gradients of either type, in one group: the same bits as each tensor in an optimizer of its own,
+    and the step of the 64-bit restatement"""
+    n = [300, 4097, 1, 256, 9000, 255, 64, 5000, 0, 0, 0, 0]
+    pd, gd = [(F32, F32, BF16, BF16)[k % 4] for k in range(12)], [(F32, BF16)[k % 2] for k in range(12)]
+    vals = [tensors([k], d, shift, 11 + i, 0.05)[0][0] for i, (k, d) in enumerate(zip(n, pd))]
+    ps, qs = [torch.nn.Parameter(v.clone()) for v in vals], [torch.nn.Parameter(v.clone()) for v in vals]
+    for p, q, d in zip(ps, qs, gd):
+        p.grad_dtype = q.grad_dtype = d
+    opt = O.MultiAdamW(ps, lr=1e-3, weight_decay=0.1, state_bits=bits)
+    each = [O.MultiAdamW([q], lr=1e-3, weight_decay=0.1, state_bits=bits) for q in qs]
+    for t in range(1, 5):
+        gs = [tensors([k], d, shift, 100 * t + i, 0.3)[0][0] for i, (k, d) in enumerate(zip(n, gd))]
+        for p, q, g in zip(ps, qs, gs):
+            p.grad, q.grad = g, g
+        before, m0, v0 = opt.flat_master().clone(), *(x.float().clone() for x in opt.flat_moments())
+        opt.step(max_norm=0.5 if clip else None)
+        norm = R.norm([np64(g) for g in gs])
+        coef = R.coefficient(norm, 0.5) if clip else 1.0
+        if clip:
+            assert abs(float(opt.grad_norm) - norm) <= 1.01 * R.EPS24 * norm
+        after, (m1, v1), at = opt.flat_master(), opt.flat_moments(), 0
+        for k, (p, q, o) in enumerate(zip(ps, qs, each)):
+            own = slice(at, at + n[k])
+            (want, wm, wv), (dp, dm, dv) = R.adamw(np64(before[own]), np64(gs[k]), np64(m0[own]), np64(v0[own]), t, lr=1e-3, wd=0.1, coef=coef)
+            within(after[own], want, dp, ("parameter", k, t))
+            if bits == 32:
+                within(m1[own], wm, dm, ("exp_avg", k, t))
+                within(v1[own], wv, dv, ("exp_avg_sq", k, t))
+            if pd[k] is F32:
+                assert torch.equal(p.detach(), after[own])
+            else:
+                half = (p.detach().float() - after[own]).abs()
+                assert bool((half <= after[own].abs() * 2.0 ** -8).all())
+            o.grad_mul = coef       # rounded to fp32 on the way in, as the clip's coefficient is
+            o.step()
+            assert torch.equal(p, q), (k, t)
+            mk, vk = o.flat_moments()
+            assert torch.equal(m1[own], mk[:n[k]]) and torch.equal(v1[own], vk[:n[k]]) and torch.equal(after[own], o.flat_master()[:n[k]])
+            end = at + -(-n[k] // 256) * 256
+            assert not any(bool(x[at + n[k]:end].float().any()) for x in (m1, v1, after)), "padding was written"
+            at = end
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_all_pairs_of_types_past_the_caches(O, bits):
+    """a call above 96 MB goes past the caches, those of its tensors alone do not: the same bits, read-outs included"""
+    n = [3_400_003, 3_400_000, 3_399_999, 3_400_257]
+    pd, gd = (F32, F32, BF16, BF16), (F32, BF16, F32, BF16)
+    gen = torch.Generator(DEV).manual_seed(3)
+    vals = [(torch.randn(k, device=DEV, generator=gen) * 0.05).to(d) for k, d in zip(n, pd)]
+    ps, qs = [torch.nn.Parameter(v.clone()) for v in vals], [torch.nn.Parameter(v.clone()) for v in vals]
+    for p, q, d in zip(ps, qs, gd):
+        p.grad_dtype = q.grad_dtype = d
+    opt, each = O.MultiAdamW(ps, lr=1e-3, state_bits=bits), [O.MultiAdamW([q], lr=1e-3, state_bits=bits) for q in qs]
+    for _ in range(2):
+        for k, d, p, q in zip(n, gd, ps, qs):
+            p.grad = torch.randn(k, device=DEV, generator=gen).to(d)
+            q.grad = p.grad
+        opt.step()
+        for o in each:
+            o.step()
+    m, v, w = *opt.flat_moments(), opt.flat_master()
+    at = 0
+    for p, q, o in zip(ps, qs, each):
+        end = at + o.flat_master().numel()
+        assert torch.equal(p, q) and torch.equal(w[at:end], o.flat_master())
+        assert torch.equal(m[at:end], o.flat_moments()[0]) and torch.equal(v[at:end], o.flat_moments()[1])
+        at = end
+    assert at == w.numel()

@@ -54,9 +54,10 @@ namespace vae {
 // own reads (past the caches: step of 69.8 M 385 against 343), and bf16 parameters, whose accesses are half as wide (151 against 147).
 #define MT_STREAM_BYTES 96e6
 
-// Up to this many chunks (four workgroups per CU, all of them running at once) a step without a norm is one launch: 39 k parameters in 8
-// tensors 8.7 us as called from Python against 12.4.  Above, waiting for its numbers in every workgroup costs more than the launch
-// that prepares them: 69.8 M parameters with 8-bit moments 212 us against 185.
+// Up to this many chunks (four workgroups per CU, all of them running at once) a step without a norm is one launch.  Above, waiting for
+// its numbers in every workgroup costs more than the launch that prepares them.  As called from Python, one launch / two, us, 30 tensors of
+// together 35 chunks 9.4 / 13.3, 266: 11.4 / 13.9, 996: 21.8 / 23.4, 1970: 41.6 / 42.0, 3921: 75.0 / 72.8; with 8-bit moments 9.3 / 13.5,
+// 9.6 / 13.6, 17.0 / 19.6, 28.9 / 27.6, 49.5 / 45.3.
 #define MT_OWN_CHUNKS 1024
 
 struct MtJob {
@@ -250,7 +251,8 @@ __device__ __forceinline__ void prep_tensors(const MtTable& tab, const MtPrep& h
     }
 }
 // A small step without a norm has no such launch: every workgroup works the numbers out for itself.  The count may advance once all
-// of the tensor's workgroups have read it: they are counted (word 7 of the slot's scalars), and the last one writes it.
+// of the tensor's workgroups have read it: they are counted (word 7 of the slot's scalars), and the last one writes it.  Called once in a
+// workgroup: a list this small has one for every chunk.
 __device__ __forceinline__ MtScal own_numbers(const MtPrep& h, uint32_t slot, uint32_t chunks) {
     __shared__ MtScal shared;
     if (threadIdx.x == 0) {
@@ -264,9 +266,7 @@ __device__ __forceinline__ MtScal own_numbers(const MtPrep& h, uint32_t slot, ui
         shared = step_numbers(h, t);
     }
     __syncthreads();
-    const MtScal s = shared;
-    __syncthreads();
-    return s;
+    return shared;
 }
 
 // workgroups 0..nsum-1: partial sums; with PREP one more, which prepares the step of the same tensors
@@ -422,7 +422,7 @@ __device__ __forceinline__ void split_master(float w, bf16_t& p, short& r) {
 // 5.7 TB/s.
 //
 // In 8 bits the vector instructions count: 16 bytes a parameter at 5.9 TB/s leave about 100 of them.  The first form took
-// 110 a parameter and 240 us, this one 65 (bf16: 77).  So
+// 110 a parameter and 240 us, this one 65 (bf16: 78).  So
 // - root and reciprocal are the hardware's, 1 ulp each, of a step that is itself a small part of the parameter.  The hardware takes
 //   the root of a subnormal for 0, which nobody sees next to an eps of at least 1e-12 (VAE_MT_MIN_EPS8): smaller ones are refused;
 // - values that are not finite, their codes, and fp32's last level are looked after in branches that a wave seldom takes;
@@ -774,9 +774,6 @@ static double elem_count(const MtTable& t) {
     for (int k = 0; k < t.count; ++k) n += (double)t.job[k].n;
     return n;
 }
-#ifndef AD_GRID
-#define AD_GRID 1048576u
-#endif
 // bytes a step's launch moves: gradient read, parameter (and remainder) and moments both ways
 static double step_bytes(const MtTable& t, bool eight) {
     double b = 0;
@@ -784,7 +781,8 @@ static double step_bytes(const MtTable& t, bool eight) {
         b += (double)t.job[k].n * (((t.job[k].slot_flags & VAE_MT_GRAD_BF16) ? 2 : 4) + 8 + (eight ? 4 : 16));
     return b;
 }
-static int update_grid(uint32_t nchunk) { return nchunk < AD_GRID ? (int)nchunk : (int)AD_GRID; }
+// a workgroup per chunk; beyond 4.3 G elements they take several
+static int update_grid(uint32_t nchunk) { return nchunk < (1u << 20) ? (int)nchunk : 1 << 20; }
 
 // sum-of-squares launches over a list (with `prep`: the step is prepared by the same launches; without `partial`: that alone); adds
 // the number of their partial sums to *np

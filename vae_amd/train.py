@@ -256,8 +256,8 @@ def fit(model, optimizer, config, train_feed, val_feed, log=None, checkpoint_pat
     ``train_feed`` / ``val_feed`` are iterables of device batches (``vae_amd.data.DeviceFeed``, or a DataLoader
     whose batches are moved with ``.to(device)``; ``(inputs, label)`` pairs are accepted).  The per-batch losses
     stay on the device and are read once per epoch (the reference's ``loss.item()`` every step stalls the stream;
-    the numbers are the same).  ``fused=True`` runs ``FusedStep`` (requires ``FlatAdamW``); otherwise the
-    autograd ``train_step``."""
+    the numbers are the same).  ``fused=True`` runs ``FusedStep`` (with ``FlatAdamW``, ``MultiAdamW`` or an optimizer of torch's);
+    otherwise the autograd ``train_step``."""
     import torch.distributed as dist
     from .data import save_checkpoint
     from .dp import sync_bn_stats

@@ -445,3 +445,47 @@ def test_all_pairs_of_types_past_the_caches(O, bits):
         assert torch.equal(m[at:end], o.flat_moments()[0]) and torch.equal(v[at:end], o.flat_moments()[1])
         at = end
     assert at == w.numel()
+
+
+# ------------------------------------------------------------------------------------------------ graphs
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_steps_with_and_without_a_norm_of_one_optimizer(O, bits):
+    """a small step without a norm counts its workgroups in the state's scratch, one with a norm leaves numbers there: two graphs of one
+    optimizer and eager steps in between, in turn, against an optimizer that only steps eagerly"""
+    n = [700, 64, 9000, 0]
+    vals, _, _ = tensors(n, F32, 0, 4, 0.1)
+    ps, qs = [torch.nn.Parameter(v.clone()) for v in vals], [torch.nn.Parameter(v.clone()) for v in vals]
+    a, b = O.MultiAdamW(ps, lr=1e-3, state_bits=bits), O.MultiAdamW(qs, lr=1e-3, state_bits=bits)
+    static = [torch.zeros_like(v) for v in vals]
+    for p, q, g in zip(ps, qs, static):
+        p.grad, q.grad = g, g
+    plain, clipped = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(plain):
+        a.step()
+    with torch.cuda.graph(clipped):
+        a.step(max_norm=1.0)
+    for t, kind in enumerate(["plain", "plain", "clipped", "eager", "plain", "clipped", "clipped", "eager clipped", "plain"]):
+        for g, new in zip(static, tensors(n, F32, 0, 70 + t)[0]):
+            g.copy_(new)
+        norm = 1.0 if "clipped" in kind else None
+        if "eager" in kind:
+            a.step(max_norm=norm)
+        else:
+            (clipped if norm else plain).replay()
+        b.step(max_norm=norm)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs)), (t, kind)
+    assert same(everything(a), everything(b)) and [int(x) for x in a._groups[0].steps] == [9] * 4
+
+
+def test_a_tensor_lr_is_filled_by_a_loaded_state(O):
+    """a captured step reads that tensor, so it stays the one it is"""
+    lr = torch.tensor(1e-3, device=DEV)
+    p = torch.nn.Parameter(torch.ones(300, device=DEV))
+    opt = O.MultiAdamW([p], lr=lr)
+    sd = copy.deepcopy(opt.state_dict())
+    sd["param_groups"][0]["lr"] = 0.5
+    opt.load_state_dict(sd)
+    assert opt.param_groups[0]["lr"] is lr and float(lr) == 0.5
+    opt.load_state_dict(opt.state_dict())
+    assert opt.param_groups[0]["lr"] is lr and float(lr) == 0.5

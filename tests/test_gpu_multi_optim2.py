@@ -489,3 +489,17 @@ def test_a_tensor_lr_is_filled_by_a_loaded_state(O):
     assert opt.param_groups[0]["lr"] is lr and float(lr) == 0.5
     opt.load_state_dict(opt.state_dict())
     assert opt.param_groups[0]["lr"] is lr and float(lr) == 0.5
+
+
+def test_a_state_loaded_on_another_stream_is_recorded_there(O, monkeypatch):
+    """the allocator learns of that stream's writes, so that the state of an optimizer that is dropped right away is not handed on before them"""
+    seen, stream = [], torch.cuda.Stream()
+    monkeypatch.setattr(O._GroupState, "used_on", lambda self, s: seen.append((self, s)))
+    _, opt = stepped(O, [300], F32, 8)
+    sd = copy.deepcopy(opt.state_dict())
+    stream.wait_stream(torch.cuda.current_stream())
+    seen.clear()
+    with torch.cuda.stream(stream):
+        opt.load_state_dict(sd)
+    torch.cuda.current_stream().wait_stream(stream)
+    assert (opt._groups[0], stream.cuda_stream) in seen

@@ -537,6 +537,7 @@ class MultiAdamW(torch.optim.Optimizer):
             self._check_group({**g, **new})
             merged.append(new)
         for new, g, st, row in zip(merged, self.param_groups, self._groups, entries):
+            st.used_on(_lib.current_stream())
             for key, x in new.items():
                 if key in ("lr", "initial_lr") and isinstance(g.get(key), torch.Tensor):
                     g[key].fill_(x)       # a captured step reads this tensor
